@@ -463,6 +463,144 @@ alphasparseStatus_t alphasparseMgGetUniqueId(void* id128);
 alphasparseStatus_t alphasparseMgCommInitRank(void** ncclComm, int world, const void* id128, int rank);
 alphasparseStatus_t alphasparseMgCommDestroy(void* ncclComm);
 
+/* ---- experts: a routing matrix and block-diagonal products (extension) ------------------- *
+ * The sparse matrices of a mixture-of-experts layer; no counterpart in the reference.
+ *
+ * The ROUTING MATRIX is tokens x experts with exactly topk entries per row: entry j of row t sits
+ * in column expertIds[t*topk + j] (a slot) and its value is the gate weight of that slot.
+ * alphasparseRoutingSort builds its column-wise form: slots in expert order, and within an expert
+ * in ascending slot number (a stable sort, the same result on every run).  A slot whose id is
+ * outside [0, experts) is dropped: it has no sorted row (a padding token, another rank's expert).
+ *   expertOffsets[e] .. expertOffsets[e+1]  the sorted rows of expert e (experts+1 offsets, I32)
+ *   position[t*topk + j]                    the slot's sorted row, or -1 for a dropped slot (I32)
+ * The EXPERT PRODUCT multiplies by a block-diagonal matrix: the rows of X are cut into segments by
+ * offsets like expertOffsets, and segment e is multiplied by dense block e.  One segment (offsets
+ * NULL) is a plain dense layer.
+ *
+ * Conventions: matrices are row-major (ALPHASPARSE_ORDER_ROW) with any leading dimension; sums,
+ * activations and statistics are fp32 and every output is rounded once; work is stream-ordered on
+ * handle->stream, nothing allocates or synchronises (alphasparseGetDeviceError apart), so calls can be captured into a graph; the
+ * handle's device is made current for the call and the caller's put back.  Outputs may not overlap
+ * inputs except where a call says so.  Sizes: rows below 2^31 - 1024, columns below 2^30.  A workspace belongs to one call at a time: calls (and
+ * captured graphs) that may run at once need one each; its contents need not be kept or cleared.
+ * Rows behind the last segment, and rows that no slot maps to, are neither read as numbers nor
+ * written.  Results do not depend on the order in which blocks run. */
+typedef enum {
+  ALPHASPARSE_ACT_NONE = 0,
+  ALPHASPARSE_ACT_RELU = 1, /* z > 0 ? z : 0 (NaN gives NaN) */
+  ALPHASPARSE_ACT_GELU = 2, /* z * Phi(z), the exact (erf) form */
+  ALPHASPARSE_ACT_SILU = 3  /* z / (1 + exp(-z)) */
+} alphasparseActivation_t;
+#define ALPHASPARSE_MAX_EXPERTS 1024
+#define ALPHASPARSE_MAX_TOPK 64
+
+struct _alphasparse_routing_descr {
+  bool init;
+  int64_t tokens, topk, experts;
+  const void* expert_ids;
+  alphasparseIndexType_t id_type;
+  int32_t* expert_offsets;
+  int32_t* position;
+};
+typedef struct _alphasparse_routing_descr* alphasparseRoutingDescr_t;
+/* Captures DEVICE pointers: expertIds[tokens*topk] (I32 or I64; read by alphasparseRoutingSort
+ * only, may be NULL for a routing that is already sorted), expertOffsets[experts+1], position
+ * [tokens*topk].  INVALID_SIZE: experts outside [1, ALPHASPARSE_MAX_EXPERTS], topk outside
+ * [1, ALPHASPARSE_MAX_TOPK], tokens*topk of 2^31 - 1 or more. */
+alphasparseStatus_t alphasparseCreateRouting(alphasparseRoutingDescr_t* descr, int64_t tokens,
+                                             int64_t topk, int64_t experts, const void* expertIds,
+                                             alphasparseIndexType_t idType, int32_t* expertOffsets,
+                                             int32_t* position);
+alphasparseStatus_t alphasparseDestroyRouting(alphasparseRoutingDescr_t descr);
+/* Fills expertOffsets and position from expertIds. */
+alphasparseStatus_t alphasparseRoutingSort(alphasparseHandle_t handle,
+                                           alphasparseRoutingDescr_t routing, void* externalBuffer);
+alphasparseStatus_t alphasparseRoutingSort_bufferSize(alphasparseHandle_t handle,
+                                                      alphasparseRoutingDescr_t routing,
+                                                      size_t* bufferSize);
+/* Tokens to experts: Xs[position[t,j]] = X[t].  X: tokens rows; Xs: up to tokens*topk rows (a
+ * position outside Xs is passed over); both R_32F, R_16F or R_16BF. */
+alphasparseStatus_t alphasparseRoutingDispatch(alphasparseHandle_t handle,
+                                               alphasparseRoutingDescr_t routing,
+                                               alphasparseDnMatDescr_t matX,
+                                               alphasparseDnMatDescr_t matXs);
+/* Experts back to tokens: Y[t] = sum_j weights[t,j] * Ys[position[t,j]] + R[t], the terms in the
+ * order of j, dropped slots left out.  weights: DEVICE float[tokens*topk], NULL for ones (then it
+ * is the gradient of alphasparseRoutingDispatch); matR: NULL for none; Y may be R. */
+alphasparseStatus_t alphasparseRoutingCombine(alphasparseHandle_t handle,
+                                              alphasparseRoutingDescr_t routing,
+                                              alphasparseDnMatDescr_t matYs, const float* weights,
+                                              alphasparseDnMatDescr_t matR,
+                                              alphasparseDnMatDescr_t matY);
+/* Gradient of alphasparseRoutingCombine (that of R is dY itself):
+ *   dYs[position[t,j]] = weights[t,j] * dY[t]            (matdYs NULL: not wanted)
+ *   dWeights[t,j]      = <dY[t], Ys[position[t,j]]>      (NULL: not wanted; 0 for a dropped slot)
+ * dYs may be Ys. */
+alphasparseStatus_t alphasparseRoutingCombineGrad(alphasparseHandle_t handle,
+                                                  alphasparseRoutingDescr_t routing,
+                                                  alphasparseDnMatDescr_t matdY,
+                                                  alphasparseDnMatDescr_t matYs, const float* weights,
+                                                  alphasparseDnMatDescr_t matdYs, float* dWeights);
+/* The experts' products with their epilogue, for the rows p of every segment e:
+ *   Z[p] = X[p] * op(W_e) + bias[e]     (matZ NULL: Z is not kept)
+ *   Y[p] = act(Z[p]) + R[p]
+ * matX: rows x K.  matW: the blocks one under the other - opW TRANSPOSE: W_e is N x K (the layout of
+ * a linear layer's weight), matW (segments*N) x K; NON_TRANSPOSE: W_e is K x N, matW (segments*K) x N.
+ * matBias: segments x N or NULL; matR: rows x N or NULL.  X and W: R_16BF or R_16F, the same; Y: that
+ * type or R_32F; Z and R: Y's type; bias: X's type or R_32F.  Y may be R.  segOffsets: DEVICE
+ * int32[segments+1], ascending, clamped to the rows of X; NULL: one segment of all rows.  fp32
+ * accumulation on the tensor cores.  K = 0 is an empty sum.
+ * The gradient with respect to X is this call on dZ with the other opW (no bias, no activation).
+ * externalBuffer: alphasparseExpertMM_bufferSize bytes (0 for the usual operands: 16-byte aligned
+ * X and W with leading dimensions that are multiples of 8; others are copied into it first). */
+alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t handle, alphasparseOperation_t opW,
+                                        int64_t segments, const int32_t* segOffsets,
+                                        alphasparseDnMatDescr_t matX, alphasparseDnMatDescr_t matW,
+                                        alphasparseDnMatDescr_t matBias, alphasparseActivation_t act,
+                                        alphasparseDnMatDescr_t matR, alphasparseDnMatDescr_t matZ,
+                                        alphasparseDnMatDescr_t matY, void* externalBuffer);
+alphasparseStatus_t alphasparseExpertMM_bufferSize(alphasparseHandle_t handle,
+                                                   alphasparseOperation_t opW, int64_t segments,
+                                                   const int32_t* segOffsets,
+                                                   alphasparseDnMatDescr_t matX,
+                                                   alphasparseDnMatDescr_t matW,
+                                                   alphasparseDnMatDescr_t matY, size_t* bufferSize);
+/* Gradient with respect to the weights, in the layout of matW (opW as in the forward call):
+ *   TRANSPOSE: dW_e = dZ_e^T * X_e (N x K)      NON_TRANSPOSE: dW_e = X_e^T * dZ_e (K x N)
+ * over the rows of segment e; an empty segment's block is zero.  X, dZ: R_16BF or R_16F, the same;
+ * dW: that type or R_32F.  externalBuffer as in alphasparseExpertMM. */
+alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t handle, alphasparseOperation_t opW,
+                                              int64_t segments, const int32_t* segOffsets,
+                                              alphasparseDnMatDescr_t matX,
+                                              alphasparseDnMatDescr_t matdZ,
+                                              alphasparseDnMatDescr_t matdW, void* externalBuffer);
+alphasparseStatus_t alphasparseExpertMM_gradW_bufferSize(alphasparseHandle_t handle,
+                                                         alphasparseOperation_t opW, int64_t segments,
+                                                         const int32_t* segOffsets,
+                                                         alphasparseDnMatDescr_t matX,
+                                                         alphasparseDnMatDescr_t matdZ,
+                                                         alphasparseDnMatDescr_t matdW,
+                                                         size_t* bufferSize);
+/* Gradient of the epilogue: dZ[p] = dY[p] * act'(Z[p]) and dBias[e] = the sum of the unrounded
+ * dZ[p] over segment e (0 for an empty one).  matdY, matZ, matdZ: rows x N, one type (R_32F, R_16F or
+ * R_16BF); dZ may be dY or Z, or NULL when only dBias is wanted; Z may be NULL with ACT_NONE.
+ * matdBias: segments x N, R_32F, or NULL (then no externalBuffer is needed).  The gradient with
+ * respect to R is dY. */
+alphasparseStatus_t alphasparseExpertActGrad(alphasparseHandle_t handle, int64_t segments,
+                                             const int32_t* segOffsets, alphasparseActivation_t act,
+                                             alphasparseDnMatDescr_t matdY, alphasparseDnMatDescr_t matZ,
+                                             alphasparseDnMatDescr_t matdZ,
+                                             alphasparseDnMatDescr_t matdBias, void* externalBuffer);
+alphasparseStatus_t alphasparseExpertActGrad_bufferSize(alphasparseHandle_t handle, int64_t segments,
+                                                        const int32_t* segOffsets,
+                                                        alphasparseActivation_t act,
+                                                        alphasparseDnMatDescr_t matdY,
+                                                        alphasparseDnMatDescr_t matdBias,
+                                                        size_t* bufferSize);
+/* 1 in *flag if a kernel of the expert products ever gave up a bounded wait on this handle (its
+ * results are then incomplete), else 0.  Synchronises handle->stream. */
+alphasparseStatus_t alphasparseGetDeviceError(alphasparseHandle_t handle, int* flag);
+
 /* ---- the step before the path: MatrixMarket file -> COO (host) ------------------------- */
 /* cuda/test/io.cu:1227-1238 (alpha_read_coo<T>(file, &m, &n, &nnz, &row_index, &col_index,
  * &values)), MatrixMarket part (:103-184, :490-575).  Reads a coordinate file into HOST arrays

@@ -29,6 +29,8 @@ INDEX_I32, INDEX_I64 = 2, 3
 BASE_ZERO, BASE_ONE = 0, 1
 SPMV_ALG_DEFAULT, SPMV_ALG_COO, SPMV_ALG_VECTOR, SPMV_ALG_MERGE = 0, 1, 6, 9
 SPMM_ALG_DEFAULT, SPMM_CSR_ALG1, SPMM_CSR_ALG2, SPMM_CSR_ALG3, SPMM_CSR_ALG4, SPMM_CSR_ALG5, SPMM_CSR_ALG6 = 0, 5, 6, 7, 8, 9, 10
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+MAX_EXPERTS, MAX_TOPK = 1024, 64
 MG_X_BROADCAST, MG_X_ALLGATHER, MG_X_WINDOW, MG_X_WINDOW_OVERLAP = 0, 1, 2, 3
 MG_INFO_NAMES = ["window_lo", "window_hi", "bytes_received", "interior_begin", "interior_end", "num_sends",
                  "num_recvs", "mode"]
@@ -50,6 +52,11 @@ EXPORTS = [
     "alphasparseMgCreate", "alphasparseMgDestroy", "alphasparseMgSetShard", "alphasparseMgSpMV",
     "alphasparseMgExchange", "alphasparseMgOwnView", "alphasparseMgGetInfo", "alphasparseMgExchangePlan",
     "alphasparseMgGetUniqueId", "alphasparseMgCommInitRank", "alphasparseMgCommDestroy",
+    "alphasparseCreateRouting", "alphasparseDestroyRouting", "alphasparseRoutingSort", "alphasparseRoutingSort_bufferSize",
+    "alphasparseRoutingDispatch", "alphasparseRoutingCombine", "alphasparseRoutingCombineGrad",
+    "alphasparseExpertMM", "alphasparseExpertMM_bufferSize", "alphasparseExpertMM_gradW",
+    "alphasparseExpertMM_gradW_bufferSize", "alphasparseExpertActGrad", "alphasparseExpertActGrad_bufferSize",
+    "alphasparseGetDeviceError",
 ]
 
 
@@ -391,6 +398,150 @@ def read_mtx(path: str, dtype=torch.float32, ordered: bool = True):
         for p in (ri, ci, v):
             lib.alphasparseFreeHost(p)
     return m.value, n.value, torch.from_numpy(rows_i), torch.from_numpy(cols_i), torch.from_numpy(vals)
+
+
+# ---- experts: routing matrix and block-diagonal products ------------------------------------
+
+class Routing:
+    """alphasparseRoutingDescr_t: ``expert_ids`` (tokens x topk, int32 or int64) chooses each token's experts; an id
+    outside [0, experts) drops the slot.  ``offsets`` (experts + 1) and ``position`` (tokens x topk), both int32, are
+    filled by ``routing_sort``; they are allocated here unless given."""
+
+    def __init__(self, expert_ids: torch.Tensor, experts: int, offsets: torch.Tensor | None = None,
+                 position: torch.Tensor | None = None):
+        assert expert_ids.is_cuda and expert_ids.dim() == 2 and expert_ids.is_contiguous()
+        self.tokens, self.topk, self.experts = int(expert_ids.shape[0]), int(expert_ids.shape[1]), int(experts)
+        self.expert_ids = expert_ids
+        dev = expert_ids.device
+        self.offsets = torch.empty(self.experts + 1, dtype=torch.int32, device=dev) if offsets is None else offsets
+        self.position = torch.empty(expert_ids.shape, dtype=torch.int32, device=dev) if position is None else position
+        for t, n in ((self.offsets, self.experts + 1), (self.position, expert_ids.numel())):
+            assert t.device == dev and t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n
+        self.d = C.c_void_p()
+        it = {torch.int32: INDEX_I32, torch.int64: INDEX_I64}[expert_ids.dtype]
+        _check(load().alphasparseCreateRouting(C.byref(self.d), C.c_int64(self.tokens), C.c_int64(self.topk),
+                                               C.c_int64(self.experts), C.c_void_p(expert_ids.data_ptr()), it,
+                                               C.c_void_p(self.offsets.data_ptr()),
+                                               C.c_void_p(self.position.data_ptr())), "alphasparseCreateRouting")
+
+    def __del__(self):
+        # at interpreter shutdown module globals may already be gone: then the process's exit frees the descriptor
+        if getattr(self, "d", None) and load is not None:
+            try:
+                load().alphasparseDestroyRouting(self.d)
+            except Exception:
+                pass
+
+
+def _d(m):
+    return m.d if m is not None else None
+
+
+def _ptr(t: torch.Tensor | None):
+    return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def _gates(routing: Routing, w: torch.Tensor | None):
+    """Pointer of a tokens x topk fp32 array (or NULL)."""
+    assert w is None or (w.is_cuda and w.dtype == torch.float32 and w.is_contiguous() and w.numel() == routing.tokens * routing.topk)
+    return _ptr(w)
+
+
+def _segments(offsets: torch.Tensor | None):
+    """(segments, device pointer) of int32 row offsets; None is one segment of all rows."""
+    if offsets is None:
+        return C.c_int64(1), None
+    assert offsets.is_cuda and offsets.dtype == torch.int32 and offsets.is_contiguous()
+    return C.c_int64(offsets.numel() - 1), _ptr(offsets)
+
+
+def routing_buffer_size(handle: Handle, routing: Routing) -> int:
+    size = C.c_size_t(0)
+    _check(load().alphasparseRoutingSort_bufferSize(handle.h, routing.d, C.byref(size)), "alphasparseRoutingSort_bufferSize")
+    return int(size.value)
+
+
+def routing_sort(handle: Handle, routing: Routing, buffer: torch.Tensor | None = None):
+    """Fill routing.offsets and routing.position from routing.expert_ids (asynchronous, like every call below)."""
+    _check(load().alphasparseRoutingSort(handle.h, routing.d, _ptr(buffer)), "alphasparseRoutingSort")
+
+
+def routing_dispatch(handle: Handle, routing: Routing, X: DnMat, Xs: DnMat):
+    """Xs[position[t, j]] = X[t]"""
+    _check(load().alphasparseRoutingDispatch(handle.h, routing.d, X.d, Xs.d), "alphasparseRoutingDispatch")
+
+
+def routing_combine(handle: Handle, routing: Routing, Ys: DnMat, Y: DnMat, weights: torch.Tensor | None = None,
+                    residual: DnMat | None = None):
+    """Y[t] = sum_j weights[t, j] * Ys[position[t, j]] + residual[t]; without weights the gradient of routing_dispatch."""
+    _check(load().alphasparseRoutingCombine(handle.h, routing.d, Ys.d, _gates(routing, weights), _d(residual), Y.d),
+           "alphasparseRoutingCombine")
+
+
+def routing_combine_grad(handle: Handle, routing: Routing, dY: DnMat, Ys: DnMat | None, dYs: DnMat | None,
+                         weights: torch.Tensor | None = None, dweights: torch.Tensor | None = None):
+    """dYs[position[t, j]] = weights[t, j] * dY[t] and dweights[t, j] = <dY[t], Ys[position[t, j]]>"""
+    _check(load().alphasparseRoutingCombineGrad(handle.h, routing.d, dY.d, _d(Ys), _gates(routing, weights), _d(dYs),
+                                                _gates(routing, dweights)), "alphasparseRoutingCombineGrad")
+
+
+def expert_mm_buffer_size(handle: Handle, X: DnMat, W: DnMat, Y: DnMat, offsets: torch.Tensor | None = None, op=OP_T) -> int:
+    size = C.c_size_t(0)
+    n, off = _segments(offsets)
+    _check(load().alphasparseExpertMM_bufferSize(handle.h, op, n, off, X.d, W.d, Y.d, C.byref(size)),
+           "alphasparseExpertMM_bufferSize")
+    return int(size.value)
+
+
+def expert_mm(handle: Handle, X: DnMat, W: DnMat, Y: DnMat, offsets: torch.Tensor | None = None, op=OP_T,
+              bias: DnMat | None = None, act=ACT_NONE, residual: DnMat | None = None, preact: DnMat | None = None,
+              buffer: torch.Tensor | None = None):
+    """Y[p] = act(X[p] @ op(W_e) + bias[e]) + residual[p] for the rows p of segment e; ``preact`` receives act's argument.
+    op OP_T: W stacks N x K blocks; OP_N: K x N blocks.  ``buffer``: expert_mm_buffer_size bytes (none when that is 0)."""
+    n, off = _segments(offsets)
+    _check(load().alphasparseExpertMM(handle.h, op, n, off, X.d, W.d, _d(bias), act, _d(residual), _d(preact), Y.d,
+                                      _ptr(buffer)), "alphasparseExpertMM")
+
+
+def expert_mm_grad_weight_buffer_size(handle: Handle, X: DnMat, dZ: DnMat, dW: DnMat, offsets: torch.Tensor | None = None,
+                                      op=OP_T) -> int:
+    size = C.c_size_t(0)
+    n, off = _segments(offsets)
+    _check(load().alphasparseExpertMM_gradW_bufferSize(handle.h, op, n, off, X.d, dZ.d, dW.d, C.byref(size)),
+           "alphasparseExpertMM_gradW_bufferSize")
+    return int(size.value)
+
+
+def expert_mm_grad_weight(handle: Handle, X: DnMat, dZ: DnMat, dW: DnMat, offsets: torch.Tensor | None = None, op=OP_T,
+                          buffer: torch.Tensor | None = None):
+    """dW_e = dZ_e^T X_e (OP_T) or X_e^T dZ_e (OP_N), stacked like W."""
+    n, off = _segments(offsets)
+    _check(load().alphasparseExpertMM_gradW(handle.h, op, n, off, X.d, dZ.d, dW.d, _ptr(buffer)),
+           "alphasparseExpertMM_gradW")
+
+
+def expert_act_grad_buffer_size(handle: Handle, dY: DnMat, offsets: torch.Tensor | None = None, act=ACT_NONE,
+                                dbias: DnMat | None = None) -> int:
+    size = C.c_size_t(0)
+    n, off = _segments(offsets)
+    _check(load().alphasparseExpertActGrad_bufferSize(handle.h, n, off, act, dY.d, _d(dbias), C.byref(size)),
+           "alphasparseExpertActGrad_bufferSize")
+    return int(size.value)
+
+
+def expert_act_grad(handle: Handle, dY: DnMat, Z: DnMat | None, dZ: DnMat | None, offsets: torch.Tensor | None = None,
+                    act=ACT_NONE, dbias: DnMat | None = None, buffer: torch.Tensor | None = None):
+    """dZ = dY * act'(Z) and dbias[e] = column sums of dZ over segment e.  ``buffer``: needed with dbias."""
+    n, off = _segments(offsets)
+    _check(load().alphasparseExpertActGrad(handle.h, n, off, act, dY.d, _d(Z), _d(dZ), _d(dbias), _ptr(buffer)),
+           "alphasparseExpertActGrad")
+
+
+def device_error(handle: Handle) -> int:
+    """1 if an expert kernel ever gave up a bounded wait on this handle (synchronises)."""
+    flag = C.c_int(0)
+    _check(load().alphasparseGetDeviceError(handle.h, C.byref(flag)), "alphasparseGetDeviceError")
+    return int(flag.value)
 
 
 # ---- multi-GPU SpMV (alphasparseMg*) ------------------------------------------------------

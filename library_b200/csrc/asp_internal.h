@@ -41,6 +41,27 @@ struct HandleImpl {
   // sustained rates estimated from the device's own attributes (clocks, SM count, bus width):
   // what the tensor-core SpMM's density test weighs MMA work against memory traffic with
   double bf16_flops = 1.4e15, hbm_bytes = 6.5e12;
+  // device flag a kernel of the expert products raises when a bounded wait expires
+  int* dev_err = nullptr;
+};
+
+// Makes the handle's device current for a scope and puts the caller's back.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+    if (prev_ != device) status = cudaSetDevice(device);
+    else prev_ = -1;
+  }
+  ~DeviceScope() {
+    if (prev_ >= 0) cudaSetDevice(prev_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  cudaError_t status = cudaSuccess;
+
+ private:
+  int prev_ = -1;
 };
 
 // The analysis result attached to a CSR descriptor (matA->info).
@@ -163,5 +184,24 @@ alphasparseStatus_t spmm_other_run(alphasparseHandle_t h, alphasparseSpMatDescr_
 bool spmv_other_types(alphasparseDataType a, alphasparseDataType x, alphasparseDataType y, alphasparseDataType compute);
 alphasparseStatus_t spmv_other_run(alphasparseHandle_t h, alphasparseSpMatDescr_t A, const Plan* p, const void* x,
                                    void* y, alphasparseDataType y_type, const void* alpha, const void* beta);
+
+// expert_route.cu / expert_mm.cu / expert_grad.cu: checks shared by the expert calls
+inline bool expert_type(alphasparseDataType t) { return t == ALPHA_R_32F || t == ALPHA_R_16F || t == ALPHA_R_16BF; }
+// A dense operand of rows x cols (either -1: any) in row-major order.
+inline alphasparseStatus_t expert_check_mat(alphasparseDnMatDescr_t m, int64_t rows, int64_t cols) {
+  if (!m || !m->init) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  if (m->order != ALPHASPARSE_ORDER_ROW) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+  if ((rows >= 0 && m->rows != rows) || (cols >= 0 && m->cols != cols)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  // row and column numbers are 32-bit in the kernels, a tile past the end included (element offsets are 64-bit)
+  if (m->rows >= (int64_t(1) << 31) - 1024 || m->cols >= (int64_t(1) << 30)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  // an element that does not sit on a multiple of its size cannot be loaded
+  if (reinterpret_cast<uintptr_t>(m->values) & (elem_size(m->data_type) - 1)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+inline alphasparseStatus_t expert_check_segments(int64_t segments, const int32_t* off) {
+  if (segments < 1 || segments > ALPHASPARSE_MAX_EXPERTS) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  if (!off && segments != 1) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
 
 }  // namespace asp

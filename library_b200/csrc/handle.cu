@@ -83,6 +83,10 @@ alphasparseStatus_t alphasparseGetHandle(alphasparseHandle_t* handle) {
     ASP_CUDA(cudaMemcpyAsync(h->sone, &s1, sizeof s1, cudaMemcpyHostToDevice, h->stream));
     ASP_CUDA(cudaMemcpyAsync(h->done, &d1, sizeof d1, cudaMemcpyHostToDevice, h->stream));
   }
+  if (!impl(h)->dev_err) {
+    ASP_CUDA(cudaMalloc((void**)&impl(h)->dev_err, sizeof(int)));
+    ASP_CUDA(cudaMemsetAsync(impl(h)->dev_err, 0, sizeof(int), h->stream));
+  }
   asp_init_kernel<<<1, 1, 0, h->stream>>>();
   ASP_CUDA(cudaGetLastError());
   ASP_CUDA(cudaStreamSynchronize(h->stream));
@@ -94,6 +98,7 @@ alphasparseStatus_t alphasparse_destory_handle(alphasparseHandle_t h) {
   cudaFree(h->buffer);
   cudaFree(h->sone);
   cudaFree(h->done);
+  cudaFree(impl(h)->dev_err);
   for (int i = 0; i < 6; ++i)
     if (h->streams[i]) cudaStreamDestroy(h->streams[i]);
   delete impl(h);
@@ -111,6 +116,16 @@ alphasparseStatus_t alphasparseGetStream(alphasparseHandle_t h, cudaStream_t* st
   if (!h) return ALPHA_SPARSE_STATUS_INVALID_HANDLE;
   if (!stream) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   *stream = h->stream;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+alphasparseStatus_t alphasparseGetDeviceError(alphasparseHandle_t h, int* flag) {
+  if (!h) return ALPHA_SPARSE_STATUS_INVALID_HANDLE;
+  if (!flag) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  DeviceScope dev(h->device);
+  ASP_CUDA(dev.status);
+  ASP_CUDA(cudaMemcpyAsync(flag, impl(h)->dev_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream));
+  ASP_CUDA(cudaStreamSynchronize(h->stream));
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
@@ -251,6 +266,38 @@ alphasparseStatus_t alphasparseDnVecSetValues(alphasparseDnVecDescr_t d, void* v
 alphasparseStatus_t alphasparseDnMatSetValues(alphasparseDnMatDescr_t d, void* values) {
   if (!d || !values) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   d->values = values;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+alphasparseStatus_t alphasparseCreateRouting(alphasparseRoutingDescr_t* descr, int64_t tokens, int64_t topk,
+                                             int64_t experts, const void* expertIds,
+                                             alphasparseIndexType_t idType, int32_t* expertOffsets,
+                                             int32_t* position) {
+  if (!descr) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  *descr = nullptr;
+  if (tokens < 0 || topk < 1 || topk > ALPHASPARSE_MAX_TOPK || experts < 1 || experts > ALPHASPARSE_MAX_EXPERTS)
+    return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  if (tokens > ((int64_t(1) << 31) - 2) / topk) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  if (idType != ALPHA_SPARSE_INDEXTYPE_I32 && idType != ALPHA_SPARSE_INDEXTYPE_I64)
+    return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+  if (!expertOffsets || (tokens > 0 && !position)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  auto* d = new (std::nothrow) _alphasparse_routing_descr();
+  if (!d) return ALPHA_SPARSE_STATUS_ALLOC_FAILED;
+  d->init = true;
+  d->tokens = tokens;
+  d->topk = topk;
+  d->experts = experts;
+  d->expert_ids = expertIds;
+  d->id_type = idType;
+  d->expert_offsets = expertOffsets;
+  d->position = position;
+  *descr = d;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
+alphasparseStatus_t alphasparseDestroyRouting(alphasparseRoutingDescr_t d) {
+  if (!d) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  delete d;
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
