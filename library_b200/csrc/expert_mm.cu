@@ -2,118 +2,633 @@
 // in the epilogue, and the gradient with respect to the blocks.
 //   Z[p,n] = sum_k X[p,k] op(W_e)[k,n] + bias[e,n],   Y[p,n] = act(Z[p,n]) + R[p,n]   for p in segment e
 //   dW_e   = dZ_e^T X_e  (or its transpose)
-// Simple form: 64 x 64 tiles staged in shared memory as fp32, a 4 x 4 block of sums per thread.
+//
+// One persistent kernel for both.  The MMA's M side (lanes of tensor memory) is always the output's
+// contiguous dimension, its N side the output's rows: a warp of the epilogue then writes 32
+// neighbouring elements of a row, and the N of an MMA, which the instruction takes in steps of 16,
+// follows a ragged segment closely.
+#include <cuda.h>
+
 #include "expert_act.h"
 #include "expert_vec.h"
 
 namespace asp {
 namespace {
 
-constexpr int kT = 64, kTK = 16, kMmThreads = 256;
+// ---- PTX helpers --------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// Address of the same shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_u32(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+// (cluster-scope address: the CTA's own barrier or a peer's)
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait on a barrier of this CTA: false if the phase did not complete within `limit` polls.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+// One lane of the converged warp, in a form that tells the compiler that exactly one thread runs the guarded code.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(pred));
+  return pred != 0;
+}
+// TMA loads into this CTA's shared memory.  The .cta_group::2 form may complete on a barrier of either CTA of the pair.
+template <int CG>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map),
+        "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+        "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+// Shared-memory descriptor of a 128-byte-swizzled operand.  K-major: rows of 64 elements (128 bytes), groups of
+// eight rows 1,024 bytes apart.  MN-major: 64 x 64 boxes (a row of 128 bytes per k), groups of eight k 1,024
+// bytes apart, the next 64 elements one box (8,192 bytes) further.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr, uint32_t lbo_bytes) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+template <int CG>
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// The barrier (of both CTAs of a pair, at the same offset) is arrived on when the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
 
-__device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e, int segments, int rows) {
-  if (!off) return e == 0 ? 0 : rows;
+// ---- the tile kernel ----------------------------------------------------------------------------
+constexpr int kKC = 64;                        // contraction per stage: 128 bytes of a 16-bit type
+constexpr int kTileM = 128;                    // M of a CTA: lanes of tensor memory
+constexpr int kTileJ = 256;                    // N of an MMA, at most: rows of the output per tile
+constexpr int kMmStages = 6;
+constexpr int kABytes = kTileM * kKC * 2;      // 16 KB
+constexpr int kBoxBytes = 64 * 128;            // an MN-major box
+constexpr int kMmThreads = 384;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;    // two warps per quarter of the lanes, each half of the columns
+constexpr int kTmemCols = 512;                 // two accumulators of 256 columns
+// Polls of a bounded wait: seconds, and more than a tile of `chunks` stages can take.
+inline uint32_t wait_limit(int64_t chunks) { return (1u << 22) + (uint32_t)(chunks < (1 << 23) ? 128 * chunks : (1 << 30)); }
+
+// Which contraction the kernel runs.
+enum MmKind {
+  kFwdT = 0,  // M = output features (W_e stored N x K, K-major),  N = rows of the segment (X, K-major), over K
+  kFwdN = 1,  // M = output features (W_e stored K x N, MN-major), N = rows of the segment (X, K-major), over K
+  kGradW = 2  // M = columns of dW_e, N = rows of dW_e (both MN-major), over the rows of the segment
+};
+
+struct MmArgs {
+  const int32_t* off;
+  int segments, rows;
+  int m_total;        // columns of the output (contiguous)
+  int j_total;        // kGradW: rows of a block of dW
+  int k;              // kFwd*: contraction length
+  int box_rows;       // kFwd*: rows of X per TMA box
+  uint32_t types;     // operand type bits of the instruction descriptor
+  void* y;
+  int64_t ldy;
+  const void* r;
+  int64_t ldr;
+  void* z;
+  int64_t ldz;
+  const void* bias;
+  int64_t ldb;
+  int bias_type;
+  int act;
+  uint32_t limit;
+  int* err;
+};
+
+__device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e, int rows) {
   const int v = off[e];
   return v < 0 ? 0 : v > rows ? rows : v;
 }
-
-// Element types the operands may have beside X's.
-__device__ __forceinline__ float load_any(const void* p, int64_t i, alphasparseDataType t) {
-  if (t == ALPHA_R_32F) return ((const float*)p)[i];
-  return t == ALPHA_R_16F ? __half2float(((const __half*)p)[i]) : __bfloat162float(((const __nv_bfloat16*)p)[i]);
-}
-__device__ __forceinline__ void store_any(void* p, int64_t i, alphasparseDataType t, float v) {
-  if (t == ALPHA_R_32F) ((float*)p)[i] = v;
-  else if (t == ALPHA_R_16F) ((__half*)p)[i] = __float2half_rn(v);
-  else ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+template <typename T>
+__device__ __forceinline__ float load_as(const void* p, int64_t i) { return Wide<T>::up(((const T*)p)[i]); }
+__device__ __forceinline__ float load_bias(const void* p, int64_t i, int t) {
+  return t == ALPHA_R_32F ? ((const float*)p)[i] : t == ALPHA_R_16F ? load_as<__half>(p, i) : load_as<__nv_bfloat16>(p, i);
 }
 
-struct Mat {
+struct Tile {
+  int e;           // segment
+  int m0;          // first column of the output (of the CTA pair)
+  int row0, rows;  // rows of the output: first (of the whole matrix), how many
+  int width;       // N of the MMA (rows rounded up to 16)
+  int k0, klen;    // contraction range
+};
+
+// Tile t of the launch.  Whole warp; every lane gets the same answer.
+template <int KIND, int CG>
+__device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off, const int* s_tile, int mblocks, int jblocks) {
+  Tile x;
+  const int lane = threadIdx.x & 31;
+  if constexpr (KIND == kGradW) {
+    const int per = mblocks * jblocks;
+    x.e = t / per;
+    const int i = t % per, j = i / mblocks;
+    x.m0 = (i % mblocks) * (kTileM * CG);
+    const int left = a.j_total - j * kTileJ;
+    x.rows = left < kTileJ ? left : kTileJ;
+    x.row0 = j * kTileJ;  // within the block of dW
+    x.k0 = s_off[x.e];
+    x.klen = s_off[x.e + 1] > x.k0 ? s_off[x.e + 1] - x.k0 : 0;
+  } else {
+    const int j = t / mblocks;
+    x.m0 = (t % mblocks) * (kTileM * CG);
+    // the segment: the last one whose first tile is not past j (two ballots over up to 1,024 segments)
+    const unsigned hi = __ballot_sync(0xffffffffu, lane * 32 < a.segments && s_tile[lane * 32 < a.segments ? lane * 32 : 0] <= j);
+    const int blk = 31 - __clz(hi);
+    const int i = blk * 32 + lane;
+    const unsigned lo = __ballot_sync(0xffffffffu, i < a.segments && s_tile[i < a.segments ? i : 0] <= j);
+    x.e = blk * 32 + 31 - __clz(lo);
+    const int b = s_off[x.e], n = s_off[x.e + 1] - b, tiles = s_tile[x.e + 1] - s_tile[x.e];
+    // the segment's rows are spread evenly over its tiles
+    const int w = ((n + tiles - 1) / tiles + 15) & ~15;
+    const int at = (j - s_tile[x.e]) * w;
+    x.row0 = b + at;
+    x.rows = n - at < w ? n - at : w;
+    x.k0 = 0;
+    x.klen = a.k;
+  }
+  x.width = (x.rows + 15) & ~15;
+  return x;
+}
+
+template <typename TO, int ACT>
+__device__ __forceinline__ void store_columns(const MmArgs& a, const Tile& x, int m, int c0, const uint32_t (&acc)[32], bool zero,
+                                              float bias, int64_t out_row0) {
+  const int n = x.rows - c0 < 32 ? x.rows - c0 : 32;
+  TO* y = (TO*)a.y + (out_row0 + c0) * a.ldy + m;
+  TO* z = a.z ? (TO*)a.z + (out_row0 + c0) * a.ldz + m : nullptr;
+  const TO* r = a.r ? (const TO*)a.r + (out_row0 + c0) * a.ldr + m : nullptr;
+  TO res[32];
+  if (r) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (c < n) res[c] = r[c * a.ldr];
+  }
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    if (c < n) {
+      float v = (zero ? 0.f : __uint_as_float(acc[c])) + bias;
+      if (z) z[c * a.ldz] = Wide<TO>::down(v);
+      v = activate<ACT>(v);
+      if (r) v += Wide<TO>::up(res[c]);
+      y[c * a.ldy] = Wide<TO>::down(v);
+    }
+  }
+}
+
+// Warp roles: 0 TMA producer, 1 MMA issuer, 2 clearing of ragged tails (kGradW), 4-11 epilogue.
+template <int KIND, int CG, typename TO>
+__global__ void __launch_bounds__(kMmThreads, 1)
+expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ MmArgs a) {
+  constexpr int kBBytes = kTileJ / CG * kKC * 2;
+  constexpr int kStage = kABytes + kBBytes;
+  extern __shared__ unsigned char smem_raw[];
+  // swizzled tiles need a 1,024-byte aligned base; the offset is the same in both CTAs of a pair
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char* gen = smem_raw + (base - raw);
+  constexpr int kStages = CG == 2 ? kMmStages : 4;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gen + kStages * kStage);
+  const uint32_t bar0 = base + kStages * kStage;
+  const uint32_t full = bar0, empty = bar0 + 8 * kStages, tail = bar0 + 16 * kStages, acc_full = bar0 + 24 * kStages,
+                 acc_empty = acc_full + 16;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 3 * kStages + 4);
+  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+  int* s_off = s_fail + 1;                             // segments + 1
+  int* s_tile = s_off + ALPHASPARSE_MAX_EXPERTS + 1;   // segments + 1
+  __shared__ int s_warp[kMmThreads / 32];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+  const int mblocks = (a.m_total + kTileM * CG - 1) / (kTileM * CG);
+  const int jblocks = KIND == kGradW ? (a.j_total + kTileJ - 1) / kTileJ : 0;
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + 8 * i, CG);   // an arrival per CTA
+      mbar_init(empty + 8 * i, 1);
+      mbar_init(tail + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, CG * kEpiWarps);
+    }
+    *s_fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc<CG>(smem_u32(s_tmem), kTmemCols);
+  for (int i = tid; i <= a.segments; i += kMmThreads) s_off[i] = a.off ? clamp_row(a.off, i, a.rows) : (i == 0 ? 0 : a.rows);
+  __syncthreads();
+  int total;
+  if constexpr (KIND == kGradW) {
+    total = a.segments * mblocks * jblocks;
+  } else {
+    // exclusive prefix of the segments' tile counts: three consecutive segments per thread
+    constexpr int kPer = (ALPHASPARSE_MAX_EXPERTS + kMmThreads - 1) / kMmThreads;
+    int cnt[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = tid * kPer + i;
+      const int n = e < a.segments ? s_off[e + 1] - s_off[e] : 0;
+      cnt[i] = n > 0 ? (n + kTileJ - 1) / kTileJ : 0;
+      sum += cnt[i];
+    }
+    int v = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kMmThreads / 32; ++w) {
+      if (w < warp) before += s_warp[w];
+      all += s_warp[w];
+    }
+    int run = before + v - sum;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = tid * kPer + i;
+      if (e < a.segments) s_tile[e] = run;
+      run += cnt[i];
+    }
+    if (tid == 0) s_tile[a.segments] = all;
+    total = all * mblocks;
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the peer's barriers are ready
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *s_tmem;
+  const int first = (int)blockIdx.x / CG, stride = (int)gridDim.x / CG;
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---------------- producer: this CTA's half of every stage ----------------
+    int st = 0;
+    uint32_t ph = 0;
+    for (int t = first; t < total && ok; t += stride) {
+      const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+      const int m = x.m0 + (int)rank * kTileM;
+      const int half = x.width / CG;  // rows of the B operand in this CTA
+      const int j = x.row0 + (int)rank * half;
+      const int boxes = KIND == kGradW ? (half + 63) / 64 : (half + a.box_rows - 1) / a.box_rows;
+      const uint32_t bytes = kABytes + (uint32_t)(KIND == kGradW ? boxes * kBoxBytes : boxes * a.box_rows * 128);
+      for (int c = 0; c < x.klen; c += kKC) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit))) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          const uint32_t sa = base + st * kStage, sb = sa + kABytes;
+          // a last chunk that has to be cleared completes on the CTA's own barrier; warp 2 passes it on
+          const bool own = KIND == kGradW && x.klen - c < kKC && ((x.klen - c) & 15) != 0;
+          const uint32_t bar = own ? tail + 8 * st : CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st;
+          mbar_arrive_tx(own && CG == 2 ? peer_u32(bar, rank) : bar, bytes);
+          if constexpr (KIND == kFwdT) {
+            tma_3d<CG>(sa, &map_a, c, m, x.e, bar);
+          } else if constexpr (KIND == kFwdN) {
+            tma_3d<CG>(sa, &map_a, m, c, x.e, bar);
+            tma_3d<CG>(sa + kBoxBytes, &map_a, m + 64, c, x.e, bar);
+          } else {
+            tma_2d<CG>(sa, &map_a, m, x.k0 + c, bar);
+            tma_2d<CG>(sa + kBoxBytes, &map_a, m + 64, x.k0 + c, bar);
+          }
+          for (int b = 0; b < boxes; ++b) {
+            if constexpr (KIND == kGradW) tma_2d<CG>(sb + b * kBoxBytes, &map_b, j + b * 64, x.k0 + c, bar);
+            else tma_2d<CG>(sb + b * a.box_rows * 128, &map_b, c, j + b * a.box_rows, bar);
+          }
+        }
+        __syncwarp();
+        if (++st == kStages) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    // no stage is left with an arrival on its way to this CTA
+    for (int i = 0; i < kStages && ok; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit));
+      if (++st == kStages) {
+        st = 0;
+        ph ^= 1u;
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (the pair's first CTA) ----------------
+    if (rank == 0) {
+      int st = 0, n = 0;
+      uint32_t ph = 0;
+      constexpr uint32_t kMajor = KIND == kFwdN ? (1u << 15) : KIND == kGradW ? (1u << 15) | (1u << 16) : 0u;
+      const uint32_t idesc0 = (1u << 4) | a.types | kMajor | ((uint32_t)(kTileM * CG >> 4) << 24);
+      constexpr uint32_t kStepA = KIND == kFwdT ? 2u : 128u, kStepB = KIND == kGradW ? 128u : 2u;  // 16 elements of k, in 16 bytes
+      for (int t = first; t < total && ok; t += stride, ++n) {
+        const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+        const int buf = n & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * buf, (uint32_t)(((n >> 1) & 1) ^ 1), a.limit))) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + (uint32_t)buf * kTileJ, idesc = idesc0 | ((uint32_t)(x.width >> 3) << 17);
+        for (int c = 0; c < x.klen; c += kKC) {
+          if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, a.limit))) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elect_one()) {
+            const uint64_t da = umma_desc(base + st * kStage, kBoxBytes), db = umma_desc(base + st * kStage + kABytes, kBoxBytes);
+            const int left = x.klen - c, steps = left >= kKC ? kKC / 16 : (left + 15) / 16;
+            for (int s = 0; s < steps; ++s) umma<CG>(d, da + s * kStepA, db + s * kStepB, idesc, c > 0 || s > 0 ? 1u : 0u);
+            umma_commit<CG>(empty + 8 * st);
+          }
+          __syncwarp();
+          if (++st == kStages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok && elect_one()) umma_commit<CG>(acc_full + 8 * buf);
+        __syncwarp();
+      }
+    }
+  } else if (warp == 2) {
+    if constexpr (KIND == kGradW) {
+      // ---------------- ragged tails: the rows of the next segment (or none) behind the last one ----------------
+      int chunk = 0;
+      uint32_t phases = 0;  // of the tail barriers, a bit per stage
+      for (int t = first; t < total && ok; t += stride) {
+        const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+        const int chunks = (x.klen + kKC - 1) / kKC, left = x.klen - (chunks - 1) * kKC;
+        chunk += chunks;
+        if (chunks == 0 || (left & 15) == 0) continue;
+        const int st = (chunk - 1) % kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(tail + 8 * st, (phases >> st) & 1u, a.limit))) {
+          ok = false;
+          break;
+        }
+        phases ^= 1u << st;
+        const int to = (left + 15) & ~15, n16 = (to - left) * 8;   // 16-byte words per box
+        const int boxes = 2 + (x.width / CG + 63) / 64;
+        unsigned char* s = gen + st * kStage;
+        for (int i = lane; i < n16 * boxes; i += 32)  // whole rows of 128 bytes: the swizzle does not matter
+          *reinterpret_cast<uint4*>(s + (i / n16) * kBoxBytes + left * 128 + (i % n16) * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st);
+        __syncwarp();
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ---------------- epilogue: lane = column of the output, accumulator column = row ----------------
+    const int quarter = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    int n = 0;
+    for (int t = first; t < total && ok; t += stride, ++n) {
+      const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+      const int buf = n & 1;
+      const int m = x.m0 + (int)rank * kTileM + quarter * 32 + lane;
+      const bool in = m < a.m_total;
+      const float bias = a.bias && in ? load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type) : 0.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * buf, (uint32_t)((n >> 1) & 1), a.limit))) {
+        ok = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t d = tmem + (uint32_t)buf * kTileJ + ((uint32_t)(quarter * 32) << 16);
+      const int64_t out_row0 = KIND == kGradW ? (int64_t)x.e * a.j_total + x.row0 : (int64_t)x.row0;
+      for (int c0 = half * 32; c0 < x.rows; c0 += 64) {
+        uint32_t acc[32];
+        tmem_ld32(d + (uint32_t)c0, acc);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (in) switch (a.act) {
+          case ALPHASPARSE_ACT_RELU: store_columns<TO, ALPHASPARSE_ACT_RELU>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
+          case ALPHASPARSE_ACT_GELU: store_columns<TO, ALPHASPARSE_ACT_GELU>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
+          case ALPHASPARSE_ACT_SILU: store_columns<TO, ALPHASPARSE_ACT_SILU>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
+          default: store_columns<TO, ALPHASPARSE_ACT_NONE>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
+        }
+        __syncwarp();  // tensor memory is read by the converged warp
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      if (lane == 0) mbar_arrive(CG == 2 ? peer_u32(acc_empty + 8 * buf, 0) : acc_empty + 8 * buf);
+    }
+  }
+  __syncwarp();
+  if (!ok && lane == 0) *s_fail = 1;
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*s_fail) {
+    // a wait ran out: say so, and give copies and MMAs still in flight time to land before the memory goes
+    if (tid == 0) *a.err = 1;
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  if constexpr (CG == 2) cluster_sync();  // the peer's MMAs read this CTA's shared memory, its arrivals land here
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1) tmem_free<CG>(tmem, kTmemCols);
+}
+
+// ---- operands the TMA cannot take: aligned copies -----------------------------------------------
+__global__ void __launch_bounds__(256)
+expert_repack_kernel(const uint16_t* __restrict__ in, int64_t ld, uint16_t* __restrict__ out, int64_t ldo, int64_t rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; r < rows; r += (int64_t)gridDim.x * 8)
+#pragma unroll 8
+    for (int c = lane; c < cols; c += 32) out[r * ldo + c] = in[r * ld + c];
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeTiledFn>(p)
+               : nullptr;
+  }();
+  return fn;
+}
+
+// A 16-bit operand ready for the TMA: base on 16 bytes, rows a multiple of 16 bytes apart.
+struct Operand {
   void* p;
-  int64_t ld;
+  int64_t rows, cols, ld;
   alphasparseDataType type;
 };
-Mat mat(alphasparseDnMatDescr_t m) { return m ? Mat{m->values, m->ld, m->data_type} : Mat{nullptr, 0, ALPHA_R_32F}; }
-
-__device__ __forceinline__ float activate_any(float z, int act) {
-  switch (act) {
-    case ALPHASPARSE_ACT_RELU: return activate<ALPHASPARSE_ACT_RELU>(z);
-    case ALPHASPARSE_ACT_GELU: return activate<ALPHASPARSE_ACT_GELU>(z);
-    case ALPHASPARSE_ACT_SILU: return activate<ALPHASPARSE_ACT_SILU>(z);
-    default: return z;
-  }
+bool tma_ready(alphasparseDnMatDescr_t m) {
+  return m->rows == 0 || m->cols == 0 || ((reinterpret_cast<uintptr_t>(m->values) & 15) == 0 && (m->ld & 7) == 0);
+}
+int64_t padded8(int64_t cols) { return (cols + 7) & ~(int64_t)7; }
+size_t repack_bytes(alphasparseDnMatDescr_t m) {
+  return tma_ready(m) ? 0 : (((size_t)m->rows * (size_t)padded8(m->cols) * 2 + 255) & ~(size_t)255);
+}
+size_t repack_bytes(alphasparseDnMatDescr_t a, alphasparseDnMatDescr_t b) {
+  const size_t n = repack_bytes(a) + repack_bytes(b);
+  return n ? n + 256 : 0;
+}
+alphasparseStatus_t ready_operand(alphasparseHandle_t h, alphasparseDnMatDescr_t m, unsigned char** scratch, Operand* o) {
+  *o = {m->values, m->rows, m->cols, m->ld, m->data_type};
+  if (tma_ready(m)) return ALPHA_SPARSE_STATUS_SUCCESS;
+  o->p = *scratch;
+  o->ld = padded8(m->cols);
+  *scratch += repack_bytes(m);
+  const int64_t blocks = (m->rows + 7) / 8;
+  expert_repack_kernel<<<(unsigned)(blocks < 8 * impl(h)->sm_count ? blocks : 8 * impl(h)->sm_count), 256, 0, h->stream>>>(
+      (const uint16_t*)m->values, m->ld, (uint16_t*)o->p, o->ld, m->rows, (int)m->cols);
+  ASP_CUDA(cudaGetLastError());
+  ++impl(h)->launches;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
-__global__ void __launch_bounds__(kMmThreads)
-expert_mm_kernel(Mat x, Mat w, Mat bias, Mat r, Mat z, Mat y, bool w_nk, int act, const int32_t* __restrict__ off,
-                 int segments, int rows, int n, int k) {
-  __shared__ float sx[kTK][kT + 1], sw[kTK][kT + 1];
-  int tile = (int)blockIdx.y, e = 0, lo = 0, hi = 0;
-  for (; e < segments; ++e) {
-    lo = clamp_row(off, e, segments, rows);
-    hi = clamp_row(off, e + 1, segments, rows);
-    const int tiles = hi > lo ? (hi - lo + kT - 1) / kT : 0;
-    if (tile < tiles) break;
-    tile -= tiles;
-  }
-  if (e == segments) return;
-  const int p0 = lo + tile * kT, n0 = (int)blockIdx.x * kT, tid = threadIdx.x;
-  const int ty = tid / 16, tx = tid % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < k; k0 += kTK) {
-    for (int i = tid; i < kT * kTK; i += kMmThreads) {
-      const int a = i / kTK, c = i % kTK;
-      sx[c][a] = p0 + a < hi && k0 + c < k ? load_any(x.p, (int64_t)(p0 + a) * x.ld + k0 + c, x.type) : 0.f;
-      float v = 0.f;
-      if (n0 + a < n && k0 + c < k)
-        v = w_nk ? load_any(w.p, ((int64_t)e * n + n0 + a) * w.ld + k0 + c, w.type)
-                 : load_any(w.p, ((int64_t)e * k + k0 + c) * w.ld + n0 + a, w.type);
-      sw[c][a] = v;
-    }
-    __syncthreads();
-    for (int c = 0; c < kTK; ++c)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sx[c][ty * 4 + i], sw[c][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int p = p0 + ty * 4 + i, c = n0 + tx + 16 * j;
-      if (p >= hi || c >= n) continue;
-      float v = acc[i][j];
-      if (bias.p) v += load_any(bias.p, (int64_t)e * bias.ld + c, bias.type);
-      if (z.p) store_any(z.p, (int64_t)p * z.ld + c, z.type, v);
-      v = activate_any(v, act);
-      if (r.p) v += load_any(r.p, (int64_t)p * r.ld + c, r.type);
-      store_any(y.p, (int64_t)p * y.ld + c, y.type, v);
-    }
+// blocks > 0: a third dimension over stacked blocks of rows / blocks rows each (out-of-range rows of a block read as
+// zero, not as the next block's).
+alphasparseStatus_t tensor_map(CUtensorMap* map, const Operand& o, int64_t blocks, uint32_t box_cols, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;
+  const cuuint32_t rank = blocks > 0 ? 3 : 2;
+  const int64_t per = blocks > 0 ? o.rows / blocks : o.rows;
+  const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)per, (cuuint64_t)blocks};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)o.ld * 2 * (cuuint64_t)per};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1}, ones[3] = {1, 1, 1};
+  const CUresult r = fn(map, o.type == ALPHA_R_16F ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, o.p, dims,
+                        strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ALPHA_SPARSE_STATUS_SUCCESS : ALPHA_SPARSE_STATUS_INVALID_VALUE;
 }
 
-// dW_e[a, b] = sum_p A[p, a] B[p, b]
-__global__ void __launch_bounds__(kMmThreads)
-expert_mm_grad_kernel(Mat a, Mat b, Mat dw, const int32_t* __restrict__ off, int segments, int rows, int m, int n) {
-  __shared__ float sa[kTK][kT + 1], sb[kTK][kT + 1];
-  const int e = (int)blockIdx.z, m0 = (int)blockIdx.y * kT, n0 = (int)blockIdx.x * kT, tid = threadIdx.x;
-  const int lo = clamp_row(off, e, segments, rows), hi = clamp_row(off, e + 1, segments, rows);
-  const int ty = tid / 16, tx = tid % 16;
-  float acc[4][4] = {};
-  for (int p0 = lo; p0 < hi; p0 += kTK) {
-    for (int i = tid; i < kT * kTK; i += kMmThreads) {
-      const int p = i / kT, c = i % kT;
-      sa[p][c] = p0 + p < hi && m0 + c < m ? load_any(a.p, (int64_t)(p0 + p) * a.ld + m0 + c, a.type) : 0.f;
-      sb[p][c] = p0 + p < hi && n0 + c < n ? load_any(b.p, (int64_t)(p0 + p) * b.ld + n0 + c, b.type) : 0.f;
-    }
-    __syncthreads();
-    for (int c = 0; c < kTK; ++c)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[c][ty * 4 + i], sb[c][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+uint32_t type_bits(alphasparseDataType t) { return t == ALPHA_R_16BF ? (1u << 7) | (1u << 10) : 0u; }
+
+template <int KIND, int CG, typename TO>
+alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles) {
+  constexpr int stages = CG == 2 ? kMmStages : 4;
+  constexpr size_t smem = 1024 + (size_t)stages * (kABytes + kTileJ / CG * kKC * 2) + 8 * (3 * stages + 4) + 8 +
+                          8 * (ALPHASPARSE_MAX_EXPERTS + 1);
+  auto kernel = expert_mm_kernel<KIND, CG, TO>;
+  ASP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int64_t most = impl(h)->sm_count / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
+  cfg.blockDim = dim3(kMmThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = h->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  ASP_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, a));
+  ++impl(h)->launches;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+template <int KIND, int CG>
+alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
+                              alphasparseDataType out) {
+  switch (out) {
+    case ALPHA_R_32F: return launch_mm<KIND, CG, float>(h, ma, mb, a, tiles);
+    case ALPHA_R_16F: return launch_mm<KIND, CG, __half>(h, ma, mb, a, tiles);
+    default: return launch_mm<KIND, CG, __nv_bfloat16>(h, ma, mb, a, tiles);
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = m0 + ty * 4 + i, c = n0 + tx + 16 * j;
-      if (r < m && c < n) store_any(dw.p, ((int64_t)e * m + r) * dw.ld + c, dw.type, acc[i][j]);
-    }
 }
 
 bool type16(alphasparseDataType t) { return t == ALPHA_R_16F || t == ALPHA_R_16BF; }
@@ -171,7 +686,7 @@ alphasparseStatus_t alphasparseExpertMM_bufferSize(alphasparseHandle_t h, alphas
   MmShape shape;
   const alphasparseStatus_t s = check_mm(h, op, segments, off, x, w, y, &shape);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-  *size = 0;
+  *size = repack_bytes(x, w);
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
@@ -191,15 +706,39 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   if (r && (s = expert_check_mat(r, shape.rows, shape.n)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   if (z && (s = expert_check_mat(z, shape.rows, shape.n)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   if (shape.rows == 0 || shape.n == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+  if (!buffer && repack_bytes(x, w)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
-  const dim3 grid((unsigned)((shape.n + kT - 1) / kT), (unsigned)((shape.rows + kT - 1) / kT + segments));
-  expert_mm_kernel<<<grid, kMmThreads, 0, h->stream>>>(mat(x), mat(w), mat(bias), mat(r), mat(z), mat(y),
-                                                       op == ALPHA_SPARSE_OPERATION_TRANSPOSE, (int)act, off,
-                                                       (int)segments, (int)shape.rows, (int)shape.n, (int)shape.k);
-  ASP_CUDA(cudaGetLastError());
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+  const bool nk = op == ALPHA_SPARSE_OPERATION_TRANSPOSE;
+  unsigned char* scratch = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(buffer) + 255) & ~(uintptr_t)255);
+  Operand ox, ow;
+  if ((s = ready_operand(h, x, &scratch, &ox)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  if ((s = ready_operand(h, w, &scratch, &ow)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  MmArgs a = {};
+  a.off = off;
+  a.segments = (int)segments;
+  a.rows = (int)shape.rows;
+  a.m_total = (int)shape.n;
+  a.k = (int)shape.k;
+  a.box_rows = 64;
+  a.types = type_bits(x->data_type);
+  a.y = y->values;
+  a.ldy = y->ld;
+  if (r) a.r = r->values, a.ldr = r->ld;
+  if (z) a.z = z->values, a.ldz = z->ld;
+  if (bias) a.bias = bias->values, a.ldb = bias->ld, a.bias_type = (int)bias->data_type;
+  a.act = (int)act;
+  a.limit = wait_limit(shape.k / kKC);
+  a.err = impl(h)->dev_err;
+  CUtensorMap mw = {}, mx = {};
+  if (shape.k > 0) {
+    if ((s = tensor_map(&mw, ow, segments, 64, nk ? kTileM : kKC)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    if ((s = tensor_map(&mx, ox, 0, kKC, (uint32_t)a.box_rows)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  }
+  // at most: every segment with rows ends in a tile of its own
+  const int64_t filled = segments < shape.rows ? segments : shape.rows;
+  const int64_t tiles = (shape.rows / kTileJ + filled) * ((shape.n + 2 * kTileM - 1) / (2 * kTileM));
+  return nk ? launch_mm<kFwdT, 2>(h, mw, mx, a, tiles, y->data_type) : launch_mm<kFwdN, 2>(h, mw, mx, a, tiles, y->data_type);
 }
 
 alphasparseStatus_t alphasparseExpertMM_gradW_bufferSize(alphasparseHandle_t h, alphasparseOperation_t op,
@@ -209,26 +748,44 @@ alphasparseStatus_t alphasparseExpertMM_gradW_bufferSize(alphasparseHandle_t h, 
   if (!size) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   const alphasparseStatus_t s = check_grad_w(h, op, segments, off, x, dz, dw);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-  *size = 0;
+  *size = repack_bytes(x, dz);
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
 alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparseOperation_t op, int64_t segments,
                                               const int32_t* off, alphasparseDnMatDescr_t x, alphasparseDnMatDescr_t dz,
                                               alphasparseDnMatDescr_t dw, void* buffer) {
-  const alphasparseStatus_t s = check_grad_w(h, op, segments, off, x, dz, dw);
+  alphasparseStatus_t s = check_grad_w(h, op, segments, off, x, dz, dw);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   const bool nk = op == ALPHA_SPARSE_OPERATION_TRANSPOSE;
-  alphasparseDnMatDescr_t a = nk ? dz : x, b = nk ? x : dz;
-  if (a->cols == 0 || b->cols == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+  alphasparseDnMatDescr_t m = nk ? x : dz, j = nk ? dz : x;  // columns and rows of a block of dW
+  if (m->cols == 0 || j->cols == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+  if (!buffer && repack_bytes(x, dz)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
-  const dim3 grid((unsigned)((b->cols + kT - 1) / kT), (unsigned)((a->cols + kT - 1) / kT), (unsigned)segments);
-  expert_mm_grad_kernel<<<grid, kMmThreads, 0, h->stream>>>(mat(a), mat(b), mat(dw), off, (int)segments, (int)x->rows,
-                                                            (int)a->cols, (int)b->cols);
-  ASP_CUDA(cudaGetLastError());
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+  unsigned char* scratch = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(buffer) + 255) & ~(uintptr_t)255);
+  Operand om, oj;
+  if ((s = ready_operand(h, m, &scratch, &om)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  if ((s = ready_operand(h, j, &scratch, &oj)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  MmArgs a = {};
+  a.off = off;
+  a.segments = (int)segments;
+  a.rows = (int)x->rows;
+  a.m_total = (int)m->cols;
+  a.j_total = (int)j->cols;
+  a.types = type_bits(x->data_type);
+  a.y = dw->values;
+  a.ldy = dw->ld;
+  a.limit = wait_limit(x->rows / kKC);
+  a.err = impl(h)->dev_err;
+  CUtensorMap mm = {}, mj = {};
+  if (x->rows > 0) {
+    if ((s = tensor_map(&mm, om, 0, 64, kKC)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+    if ((s = tensor_map(&mj, oj, 0, 64, kKC)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  }
+  const int64_t tiles = segments * ((m->cols + 2 * kTileM - 1) / (2 * kTileM)) * ((j->cols + kTileJ - 1) / kTileJ);
+  if (tiles >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  return launch_mm<kGradW, 2>(h, mm, mj, a, tiles, dw->data_type);
 }
 
 }  // extern "C"
