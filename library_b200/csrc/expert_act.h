@@ -1,20 +1,62 @@
 // Activations of the expert products and their slopes, in fp32.
-//   relu  z > 0 ? z : 0                slope 1 where z > 0
-//   gelu  z Phi(z) = z erfc(-z / sqrt 2) / 2    slope Phi(z) + z phi(z)
+//   relu  z < 0 ? 0 : z                slope 1 where z > 0
+//   gelu  z Phi(z)                     slope Phi(z) + z phi(z)
 //   silu  z s(z), s(z) = 1 / (1 + exp(-z))      slope s(z) + z s(z) (1 - s(z))
-// erfc keeps the relative accuracy of Phi(z) for negative z, where 1 + erf would cancel.  Far out,
-// where the formulas would multiply an infinity with a zero, the limits are taken.
+// Phi(-|z|) = phi-shaped factor exp(-z^2 / 2) times the slowly varying erfcx(|z| / sqrt 2) / 2.  The second
+// factor behaves like 1 / |z| far out, so with t = 1 / (1 + 0.26 |z|) it is t times a polynomial in t:
+// degree 8, the coefficients a reweighted least-squares fit of the relative error over 0 <= |z| <= 14.5
+// (at most 2.9e-8; beyond, exp(-z^2 / 2) is zero in fp32).  Evaluated in fp32 the absolute error of Phi is
+// at most 2e-7 and its relative error 2.2e-6 out to z = -9.  One reciprocal, one exponential and no branch: the
+// library's erfcf made the activation, not the product, the longest part of a tile (452 us against
+// 239 us for the product alone at 16 x 2,048 rows, K = N = 2,048).
+// Far out, where the formulas would multiply an infinity with a zero, the limits are taken; NaN stays NaN.
 #pragma once
 
 #include "asp_internal.h"
 
 namespace asp {
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.44269504f;
+
+// Phi(z); *e receives exp(-z^2 / 2).
+__device__ __forceinline__ float normal_cdf(float z, float* e) {
+  const float t = rcp_fast(fmaf(0.26f, fabsf(z), 1.f));
+  float q = 0.0302303012f;
+  q = fmaf(q, t, -0.151494438f);
+  q = fmaf(q, t, 0.248733209f);
+  q = fmaf(q, t, -0.147789338f);
+  q = fmaf(q, t, 0.158758764f);
+  q = fmaf(q, t, 0.0519648210f);
+  q = fmaf(q, t, 0.102788682f);
+  q = fmaf(q, t, 0.103050974f);
+  q = fmaf(q, t, 0.103757022f);
+  *e = exp2_fast((-0.5f * kLog2e) * (z * z));
+  const float below = q * t * *e;
+  return z < 0.f ? below : 1.f - below;
+}
+
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == ALPHASPARSE_ACT_RELU) return z < 0.f ? 0.f : z;
-  if constexpr (ACT == ALPHASPARSE_ACT_GELU) return z < -20.f ? 0.f : 0.5f * z * erfcf(-0.70710678f * z);
-  if constexpr (ACT == ALPHASPARSE_ACT_SILU) return z < -110.f ? 0.f : __fdividef(z, 1.f + expf(-z));
+  if constexpr (ACT == ALPHASPARSE_ACT_GELU) {
+    float e;
+    z = z < -20.f ? -20.f : z;
+    return z * normal_cdf(z, &e);
+  }
+  if constexpr (ACT == ALPHASPARSE_ACT_SILU) {
+    z = z < -120.f ? -120.f : z;
+    return z * rcp_fast(1.f + exp2_fast(-kLog2e * z));
+  }
   return z;
 }
 
@@ -22,14 +64,16 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == ALPHASPARSE_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == ALPHASPARSE_ACT_GELU) {
-    if (fabsf(z) > 20.f) return z > 0.f ? 1.f : 0.f;
-    return 0.5f * erfcf(-0.70710678f * z) + z * (0.39894228f * expf(-0.5f * z * z));
+    float e;
+    z = z < -20.f ? -20.f : z > 20.f ? 20.f : z;
+    const float p = normal_cdf(z, &e);
+    return fmaf(z, 0.398942280f * e, p);
   }
   if constexpr (ACT == ALPHASPARSE_ACT_SILU) {
-    if (fabsf(z) > 110.f) return z > 0.f ? 1.f : 0.f;
+    z = z < -120.f ? -120.f : z > 120.f ? 120.f : z;
     // e = exp(-|z|) in (0, 1]: s(z) (1 - s(z)) = e / (1 + e)^2 is symmetric in z
-    const float e = expf(-fabsf(z)), r = __fdividef(1.f, 1.f + e);
-    return (z >= 0.f ? r : e * r) + z * (e * r * r);
+    const float e = exp2_fast(-kLog2e * fabsf(z)), r = rcp_fast(1.f + e), er = e * r;
+    return fmaf(z, er * r, z < 0.f ? er : r);
   }
   return 1.f;
 }

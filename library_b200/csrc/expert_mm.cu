@@ -34,9 +34,11 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-// (cluster-scope address: the CTA's own barrier or a peer's)
+// Arrivals take a cluster address: the CTA's own barrier or a peer's.  The producer's carries no data of
+// its own (the copies complete on the barrier by themselves), so it is relaxed: a release at cluster
+// scope waits for the warp's earlier operations, once per stage.
 __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -47,7 +49,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -249,28 +251,56 @@ __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off
   return x;
 }
 
-template <typename TO, int ACT>
-__device__ __forceinline__ void store_columns(const MmArgs& a, const Tile& x, int m, int c0, const uint32_t (&acc)[32], bool zero,
-                                              float bias, int64_t out_row0) {
-  const int n = x.rows - c0 < 32 ? x.rows - c0 : 32;
-  TO* y = (TO*)a.y + (out_row0 + c0) * a.ldy + m;
-  TO* z = a.z ? (TO*)a.z + (out_row0 + c0) * a.ldz + m : nullptr;
-  const TO* r = a.r ? (const TO*)a.r + (out_row0 + c0) * a.ldr + m : nullptr;
+// The epilogue of 32 accumulator columns (rows c0 .. of the tile) for the lane's output column m.
+// FULL: all 32 rows exist.  Each optional operand is one guarded loop, not a test per element.
+template <typename TO, int ACT, bool FULL>
+__device__ __forceinline__ void finish_columns(const MmArgs& a, const Tile& x, int m, int c0, uint32_t tmem, bool in, float bias,
+                                               int64_t out_row0) {
+  const int n = FULL ? 32 : x.rows - c0;
+  const int64_t row = out_row0 + c0;
   TO res[32];
-  if (r) {
+  if (a.r && in) {  // asked for before the accumulators are waited on
+    const TO* r = (const TO*)a.r + row * a.ldr + m;
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (c < n) res[c] = r[c * a.ldr];
+    for (int c = 0; c < 32; ++c, r += a.ldr)
+      if (FULL || c < n) res[c] = *r;
+  }
+  uint32_t acc[32];
+  tmem_ld32(tmem + (uint32_t)c0, acc);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  if (!in) return;
+  float v[32];
+#pragma unroll
+  for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(acc[c]) + bias;
+  if (x.klen == 0) {  // an empty sum: no MMA wrote the accumulators
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = bias;
+  }
+  if (a.z) {
+    TO* z = (TO*)a.z + row * a.ldz + m;
+#pragma unroll
+    for (int c = 0; c < 32; ++c, z += a.ldz)
+      if (FULL || c < n) *z = Wide<TO>::down(v[c]);
   }
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
-    if (c < n) {
-      float v = (zero ? 0.f : __uint_as_float(acc[c])) + bias;
-      if (z) z[c * a.ldz] = Wide<TO>::down(v);
-      v = activate<ACT>(v);
-      if (r) v += Wide<TO>::up(res[c]);
-      y[c * a.ldy] = Wide<TO>::down(v);
-    }
+  for (int c = 0; c < 32; ++c) v[c] = activate<ACT>(v[c]);
+  if (a.r) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (FULL || c < n) v[c] += Wide<TO>::up(res[c]);
+  }
+  TO* y = (TO*)a.y + row * a.ldy + m;
+#pragma unroll
+  for (int c = 0; c < 32; ++c, y += a.ldy)
+    if (FULL || c < n) *y = Wide<TO>::down(v[c]);
+}
+template <typename TO, int ACT>
+__device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int m, int half, uint32_t tmem, bool in, float bias,
+                                            int64_t out_row0) {
+  for (int c0 = half * 32; c0 < x.rows; c0 += 64) {
+    if (c0 + 32 <= x.rows) finish_columns<TO, ACT, true>(a, x, m, c0, tmem, in, bias, out_row0);
+    else finish_columns<TO, ACT, false>(a, x, m, c0, tmem, in, bias, out_row0);
+    __syncwarp();  // tensor memory is read by the converged warp
   }
 }
 
@@ -435,6 +465,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             ok = false;
             break;
           }
+          // (zeros that a warp of the peer stored in its tail)
+          if (KIND == kGradW && CG == 2 && x.klen - c < kKC) asm volatile("fence.acq_rel.cluster;" ::: "memory");
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (elect_one()) {
             const uint64_t da = umma_desc(base + st * kStage, kBoxBytes), db = umma_desc(base + st * kStage + kABytes, kBoxBytes);
@@ -496,17 +528,11 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t d = tmem + (uint32_t)buf * kTileJ + ((uint32_t)(quarter * 32) << 16);
       const int64_t out_row0 = KIND == kGradW ? (int64_t)x.e * a.j_total + x.row0 : (int64_t)x.row0;
-      for (int c0 = half * 32; c0 < x.rows; c0 += 64) {
-        uint32_t acc[32];
-        tmem_ld32(d + (uint32_t)c0, acc);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (in) switch (a.act) {
-          case ALPHASPARSE_ACT_RELU: store_columns<TO, ALPHASPARSE_ACT_RELU>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
-          case ALPHASPARSE_ACT_GELU: store_columns<TO, ALPHASPARSE_ACT_GELU>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
-          case ALPHASPARSE_ACT_SILU: store_columns<TO, ALPHASPARSE_ACT_SILU>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
-          default: store_columns<TO, ALPHASPARSE_ACT_NONE>(a, x, m, c0, acc, x.klen == 0, bias, out_row0); break;
-        }
-        __syncwarp();  // tensor memory is read by the converged warp
+      switch (KIND == kGradW ? ALPHASPARSE_ACT_NONE : a.act) {
+        case ALPHASPARSE_ACT_RELU: finish_tile<TO, ALPHASPARSE_ACT_RELU>(a, x, m, half, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_GELU: finish_tile<TO, ALPHASPARSE_ACT_GELU>(a, x, m, half, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_SILU: finish_tile<TO, ALPHASPARSE_ACT_SILU>(a, x, m, half, d, in, bias, out_row0); break;
+        default: finish_tile<TO, ALPHASPARSE_ACT_NONE>(a, x, m, half, d, in, bias, out_row0); break;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       if (lane == 0) mbar_arrive(CG == 2 ? peer_u32(acc_empty + 8 * buf, 0) : acc_empty + 8 * buf);
