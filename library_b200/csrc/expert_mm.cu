@@ -142,15 +142,12 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
   else
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 
@@ -251,54 +248,55 @@ __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off
   return x;
 }
 
-// The epilogue of 32 accumulator columns (rows c0 .. of the tile) for the lane's output column m.
-// FULL: all 32 rows exist.  Each optional operand is one guarded loop, not a test per element.
+constexpr int kCols = 16;  // (32 at a time spilled registers)
+// The epilogue of 16 accumulator columns (rows c0 .. of the tile) for the lane's output column m.
+// FULL: all 16 rows exist.  Each optional operand is one guarded loop, not a test per element.
 template <typename TO, int ACT, bool FULL>
 __device__ __forceinline__ void finish_columns(const MmArgs& a, const Tile& x, int m, int c0, uint32_t tmem, bool in, float bias,
                                                int64_t out_row0) {
-  const int n = FULL ? 32 : x.rows - c0;
+  const int n = FULL ? kCols : x.rows - c0;
   const int64_t row = out_row0 + c0;
-  TO res[32];
+  TO res[kCols];
   if (a.r && in) {  // asked for before the accumulators are waited on
     const TO* r = (const TO*)a.r + row * a.ldr + m;
 #pragma unroll
-    for (int c = 0; c < 32; ++c, r += a.ldr)
+    for (int c = 0; c < kCols; ++c, r += a.ldr)
       if (FULL || c < n) res[c] = *r;
   }
-  uint32_t acc[32];
-  tmem_ld32(tmem + (uint32_t)c0, acc);
+  uint32_t acc[kCols];
+  tmem_ld16(tmem + (uint32_t)c0, acc);
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
   if (!in) return;
-  float v[32];
+  float v[kCols];
 #pragma unroll
-  for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(acc[c]) + bias;
+  for (int c = 0; c < kCols; ++c) v[c] = __uint_as_float(acc[c]) + bias;
   if (x.klen == 0) {  // an empty sum: no MMA wrote the accumulators
 #pragma unroll
-    for (int c = 0; c < 32; ++c) v[c] = bias;
+    for (int c = 0; c < kCols; ++c) v[c] = bias;
   }
   if (a.z) {
     TO* z = (TO*)a.z + row * a.ldz + m;
 #pragma unroll
-    for (int c = 0; c < 32; ++c, z += a.ldz)
+    for (int c = 0; c < kCols; ++c, z += a.ldz)
       if (FULL || c < n) *z = Wide<TO>::down(v[c]);
   }
 #pragma unroll
-  for (int c = 0; c < 32; ++c) v[c] = activate<ACT>(v[c]);
+  for (int c = 0; c < kCols; ++c) v[c] = activate<ACT>(v[c]);
   if (a.r) {
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
+    for (int c = 0; c < kCols; ++c)
       if (FULL || c < n) v[c] += Wide<TO>::up(res[c]);
   }
   TO* y = (TO*)a.y + row * a.ldy + m;
 #pragma unroll
-  for (int c = 0; c < 32; ++c, y += a.ldy)
+  for (int c = 0; c < kCols; ++c, y += a.ldy)
     if (FULL || c < n) *y = Wide<TO>::down(v[c]);
 }
 template <typename TO, int ACT>
 __device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int m, int half, uint32_t tmem, bool in, float bias,
                                             int64_t out_row0) {
-  for (int c0 = half * 32; c0 < x.rows; c0 += 64) {
-    if (c0 + 32 <= x.rows) finish_columns<TO, ACT, true>(a, x, m, c0, tmem, in, bias, out_row0);
+  for (int c0 = half * kCols; c0 < x.rows; c0 += 2 * kCols) {
+    if (c0 + kCols <= x.rows) finish_columns<TO, ACT, true>(a, x, m, c0, tmem, in, bias, out_row0);
     else finish_columns<TO, ACT, false>(a, x, m, c0, tmem, in, bias, out_row0);
     __syncwarp();  // tensor memory is read by the converged warp
   }
