@@ -84,8 +84,21 @@ def load():
         lib.alphasparseGetLaunchCount.restype = C.c_int64
         lib.get_time_us.restype = C.c_double
         lib.get_avg_time_n.restype = C.c_double
+        _declare_experts(lib)
         _lib = lib
     return _lib
+
+
+def _declare_experts(lib):
+    """Argument types of the expert calls: a serving step makes several of them per layer, and ctypes converts plain
+    integers for declared arguments in a fraction of the time that wrapper objects take."""
+    p, i, n = C.c_void_p, C.c_int, C.c_int64
+    for name, args in (("alphasparseRoutingSort", [p, p, p]), ("alphasparseRoutingDispatch", [p, p, p, p]),
+                       ("alphasparseRoutingCombine", [p, p, p, p, p, p]), ("alphasparseRoutingCombineGrad", [p, p, p, p, p, p, p]),
+                       ("alphasparseExpertMM", [p, i, n, p, p, p, p, i, p, p, p, p]),
+                       ("alphasparseExpertMM_gradW", [p, i, n, p, p, p, p, p]),
+                       ("alphasparseExpertActGrad", [p, n, p, i, p, p, p, p, p])):
+        getattr(lib, name).argtypes = args
 
 
 def _check(st: int, where: str):
@@ -124,7 +137,8 @@ class Handle:
         self.use_torch_stream()
 
     def use_torch_stream(self):
-        self.set_stream(torch.cuda.current_stream().cuda_stream)
+        # the stream's number without the Stream object around it, which takes longer than a launch
+        self.set_stream(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
     def set_stream(self, cuda_stream: int):
         _check(self.lib.alphasparseSetStream(self.h, C.c_void_p(cuda_stream)), "alphasparseSetStream")
@@ -438,7 +452,7 @@ def _d(m):
 
 
 def _ptr(t: torch.Tensor | None):
-    return C.c_void_p(t.data_ptr()) if t is not None else None
+    return t.data_ptr() if t is not None else None
 
 
 def _gates(routing: Routing, w: torch.Tensor | None):
@@ -450,9 +464,9 @@ def _gates(routing: Routing, w: torch.Tensor | None):
 def _segments(offsets: torch.Tensor | None):
     """(segments, device pointer) of int32 row offsets; None is one segment of all rows."""
     if offsets is None:
-        return C.c_int64(1), None
+        return 1, None
     assert offsets.is_cuda and offsets.dtype == torch.int32 and offsets.is_contiguous()
-    return C.c_int64(offsets.numel() - 1), _ptr(offsets)
+    return offsets.numel() - 1, offsets.data_ptr()
 
 
 def routing_buffer_size(handle: Handle, routing: Routing) -> int:
@@ -488,7 +502,7 @@ def routing_combine_grad(handle: Handle, routing: Routing, dY: DnMat, Ys: DnMat 
 def expert_mm_buffer_size(handle: Handle, X: DnMat, W: DnMat, Y: DnMat, offsets: torch.Tensor | None = None, op=OP_T) -> int:
     size = C.c_size_t(0)
     n, off = _segments(offsets)
-    _check(load().alphasparseExpertMM_bufferSize(handle.h, op, n, off, X.d, W.d, Y.d, C.byref(size)),
+    _check(load().alphasparseExpertMM_bufferSize(handle.h, op, C.c_int64(n), C.c_void_p(off), X.d, W.d, Y.d, C.byref(size)),
            "alphasparseExpertMM_bufferSize")
     return int(size.value)
 
@@ -507,7 +521,7 @@ def expert_mm_grad_weight_buffer_size(handle: Handle, X: DnMat, dZ: DnMat, dW: D
                                       op=OP_T) -> int:
     size = C.c_size_t(0)
     n, off = _segments(offsets)
-    _check(load().alphasparseExpertMM_gradW_bufferSize(handle.h, op, n, off, X.d, dZ.d, dW.d, C.byref(size)),
+    _check(load().alphasparseExpertMM_gradW_bufferSize(handle.h, op, C.c_int64(n), C.c_void_p(off), X.d, dZ.d, dW.d, C.byref(size)),
            "alphasparseExpertMM_gradW_bufferSize")
     return int(size.value)
 
@@ -524,7 +538,7 @@ def expert_act_grad_buffer_size(handle: Handle, dY: DnMat, offsets: torch.Tensor
                                 dbias: DnMat | None = None) -> int:
     size = C.c_size_t(0)
     n, off = _segments(offsets)
-    _check(load().alphasparseExpertActGrad_bufferSize(handle.h, n, off, act, dY.d, _d(dbias), C.byref(size)),
+    _check(load().alphasparseExpertActGrad_bufferSize(handle.h, C.c_int64(n), C.c_void_p(off), act, dY.d, _d(dbias), C.byref(size)),
            "alphasparseExpertActGrad_bufferSize")
     return int(size.value)
 

@@ -1,6 +1,6 @@
 // Gradient of the experts' epilogue:  dZ = dY * act'(Z),  dBias[e] = column sums of the unrounded dZ over segment e.
 //
-// One pass over dY and Z.  A CTA takes a chunk of 128 rows x one stretch of columns and walks the
+// One pass over dY and Z.  A CTA takes a chunk of 256 rows x one stretch of columns and walks the
 // segments that meet the chunk; a segment's column sums stay in registers, are joined over the CTA's
 // warps through shared memory, and go to dBias at once when the segment lies inside the chunk, else
 // (a piece of it) to the workspace: slot 0 of the chunk for a segment that began earlier, slot 1 for
@@ -14,7 +14,8 @@ namespace {
 
 constexpr int kActThreads = 256;
 constexpr int kActWarps = kActThreads / 32;
-constexpr int kActRows = 128;
+constexpr int kActRows = 256;
+constexpr int kActBatch = 4;
 
 __device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e, int segments, int rows) {
   if (!off) return e == 0 ? 0 : rows;
@@ -23,7 +24,7 @@ __device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e,
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kActThreads)
+__global__ void __launch_bounds__(kActThreads, 3)
 expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz, int64_t lddz,
                        float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
                        int cols, int strips, float* __restrict__ pieces) {
@@ -45,22 +46,30 @@ expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[v] = 0.f;
     if (c < cols) {
-#pragma unroll 4
-      for (int r = lo + warp; r < hi; r += kActWarps) {
-        const Pack<T, V> g = load_pack<T, V>(dy + (int64_t)r * lddy + c);
-        float f[V];
-        if constexpr (ACT != ALPHASPARSE_ACT_NONE) {
-          const Pack<T, V> a = load_pack<T, V>(z + (int64_t)r * ldz + c);
+      // kActBatch rows are read before the first is written: dZ may be dY or Z, so the compiler cannot reorder them
+      for (int r = lo + warp; r < hi; r += kActWarps * kActBatch) {
+        Pack<T, V> g[kActBatch], a[kActBatch];
 #pragma unroll
-          // (an explicit product: the sum below takes the same value whether or not dZ is stored)
-          for (int v = 0; v < V; ++v) f[v] = __fmul_rn(Wide<T>::up(g.v[v]), act_slope<ACT>(Wide<T>::up(a.v[v])));
-        } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v) f[v] = Wide<T>::up(g.v[v]);
+        for (int i = 0; i < kActBatch; ++i) {
+          const int row = r + i * kActWarps;
+          if (row >= hi) continue;
+          g[i] = load_pack<T, V>(dy + (int64_t)row * lddy + c);
+          if constexpr (ACT != ALPHASPARSE_ACT_NONE) a[i] = load_pack<T, V>(z + (int64_t)row * ldz + c);
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += f[v];
-        if (dz) store_pack<T, V>(dz + (int64_t)r * lddz + c, round_pack<T, V>(f));
+        for (int i = 0; i < kActBatch; ++i) {
+          const int row = r + i * kActWarps;
+          if (row >= hi) continue;
+          float f[V];
+#pragma unroll
+          // (an explicit product: the sum below takes the same value whether or not dZ is stored)
+          for (int v = 0; v < V; ++v) {
+            f[v] = g[i].at(v);
+            if constexpr (ACT != ALPHASPARSE_ACT_NONE) f[v] = __fmul_rn(f[v], act_slope<ACT>(a[i].at(v)));
+            sum[v] += f[v];
+          }
+          if (dz) store_pack<T, V>(dz + (int64_t)row * lddz + c, round_pack<T, V>(f));
+        }
       }
     }
     if (!dbias) continue;
@@ -78,28 +87,29 @@ expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz
   }
 }
 
-// 32 columns of one segment's dBias per CTA: warp w adds the pieces of every eighth chunk, then the warps are joined.
+// 64 columns of one segment's dBias per CTA: quarter q of the CTA adds the pieces of every fourth chunk, then the quarters are joined.
+constexpr int kJoinCols = 64, kJoinParts = kActThreads / kJoinCols;
 __global__ void __launch_bounds__(kActThreads)
 expert_bias_join_kernel(float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
                         int cols, int strips, const float* __restrict__ pieces) {
-  __shared__ float part[kActWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int e = (int)(blockIdx.x / (unsigned)strips), c = (int)(blockIdx.x % (unsigned)strips) * 32 + lane;
+  __shared__ float part[kJoinParts][kJoinCols];
+  const int q = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
+  const int e = (int)(blockIdx.x / (unsigned)strips), c = (int)(blockIdx.x % (unsigned)strips) * kJoinCols + i;
   const int b = clamp_row(off, e, segments, rows), d = clamp_row(off, e + 1, segments, rows);
   const int k0 = b / kActRows, k1 = d > b ? (d - 1) / kActRows : k0;
   if (d > b && k0 == k1) return;  // written by the CTA of that chunk
   float sum = 0.f;
   if (d > b && c < cols) {
-#pragma unroll 4
-    for (int k = k0 + warp; k <= k1; k += kActWarps)
+#pragma unroll 8
+    for (int k = k0 + q; k <= k1; k += kJoinParts)
       sum += pieces[(int64_t)(2 * k + (b < k * kActRows ? 0 : 1)) * cols + c];
   }
-  part[warp][lane] = sum;
+  part[q][i] = sum;
   __syncthreads();
-  if (warp == 0 && c < cols) {
+  if (q == 0 && c < cols) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kActWarps; ++w) s += part[w][lane];
+    for (int w = 0; w < kJoinParts; ++w) s += part[w][i];
     dbias[(int64_t)e * lddb + c] = s;
   }
 }
@@ -125,7 +135,7 @@ alphasparseStatus_t run_act_grad(alphasparseHandle_t h, int segments, const int3
     ++impl(h)->launches;
   }
   if (db) {
-    const int64_t js = ((int64_t)cols + 31) / 32;
+    const int64_t js = ((int64_t)cols + kJoinCols - 1) / kJoinCols;
     if (segments * js >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
     expert_bias_join_kernel<<<(unsigned)(segments * js), kActThreads, 0, h->stream>>>(
         (float*)db->values, db->ld, off, segments, rows, cols, (int)js, pieces);

@@ -9,6 +9,8 @@
 // follows a ragged segment closely.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "expert_act.h"
 #include "expert_vec.h"
 
@@ -211,11 +213,64 @@ struct Tile {
   int k0, klen;    // contraction range
 };
 
+// s_tile[e] = tiles of ROWS rows of the segments before e (s_tile[segments]: of all, returned).  All THREADS of the CTA; consecutive
+// segments per thread.  s_warp: a word per warp.
+template <int THREADS, int ROWS>
+__device__ __forceinline__ int segment_tiles(const int* s_off, int segments, int* s_tile, int* s_warp) {
+  constexpr int kPer = (ALPHASPARSE_MAX_EXPERTS + THREADS - 1) / THREADS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int cnt[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = tid * kPer + i;
+    const int n = e < segments ? s_off[e + 1] - s_off[e] : 0;
+    cnt[i] = n > 0 ? (n + ROWS - 1) / ROWS : 0;
+    sum += cnt[i];
+  }
+  int v = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) s_warp[warp] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += s_warp[w];
+    all += s_warp[w];
+  }
+  int run = before + v - sum;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = tid * kPer + i;
+    if (e < segments) s_tile[e] = run;
+    run += cnt[i];
+  }
+  if (tid == 0) s_tile[segments] = all;
+  return all;
+}
+// Row tile j: its segment and rows (the segment's rows are spread evenly over its tiles).  Whole warp; every lane gets the same answer.
+__device__ __forceinline__ void row_tile(int j, int segments, const int* s_off, const int* s_tile, Tile& x) {
+  const int lane = threadIdx.x & 31;
+  // the segment: the last one whose first tile is not past j (two ballots over up to 1,024 segments)
+  const unsigned hi = __ballot_sync(0xffffffffu, lane * 32 < segments && s_tile[lane * 32 < segments ? lane * 32 : 0] <= j);
+  const int blk = 31 - __clz(hi);
+  const int i = blk * 32 + lane;
+  const unsigned lo = __ballot_sync(0xffffffffu, i < segments && s_tile[i < segments ? i : 0] <= j);
+  x.e = blk * 32 + 31 - __clz(lo);
+  const int b = s_off[x.e], n = s_off[x.e + 1] - b, tiles = s_tile[x.e + 1] - s_tile[x.e];
+  const int w = ((n + tiles - 1) / tiles + 15) & ~15;
+  const int at = (j - s_tile[x.e]) * w;
+  x.row0 = b + at;
+  x.rows = n - at < w ? n - at : w;
+}
+
 // Tile t of the launch.  Whole warp; every lane gets the same answer.
 template <int KIND, int CG>
 __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off, const int* s_tile, int mblocks, int jblocks) {
   Tile x;
-  const int lane = threadIdx.x & 31;
   if constexpr (KIND == kGradW) {
     const int per = mblocks * jblocks;
     x.e = t / per;
@@ -227,20 +282,8 @@ __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off
     x.k0 = s_off[x.e];
     x.klen = s_off[x.e + 1] > x.k0 ? s_off[x.e + 1] - x.k0 : 0;
   } else {
-    const int j = t / mblocks;
     x.m0 = (t % mblocks) * (kTileM * CG);
-    // the segment: the last one whose first tile is not past j (two ballots over up to 1,024 segments)
-    const unsigned hi = __ballot_sync(0xffffffffu, lane * 32 < a.segments && s_tile[lane * 32 < a.segments ? lane * 32 : 0] <= j);
-    const int blk = 31 - __clz(hi);
-    const int i = blk * 32 + lane;
-    const unsigned lo = __ballot_sync(0xffffffffu, i < a.segments && s_tile[i < a.segments ? i : 0] <= j);
-    x.e = blk * 32 + 31 - __clz(lo);
-    const int b = s_off[x.e], n = s_off[x.e + 1] - b, tiles = s_tile[x.e + 1] - s_tile[x.e];
-    // the segment's rows are spread evenly over its tiles
-    const int w = ((n + tiles - 1) / tiles + 15) & ~15;
-    const int at = (j - s_tile[x.e]) * w;
-    x.row0 = b + at;
-    x.rows = n - at < w ? n - at : w;
+    row_tile(t / mblocks, a.segments, s_off, s_tile, x);
     x.k0 = 0;
     x.klen = a.k;
   }
@@ -249,31 +292,20 @@ __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off
 }
 
 constexpr int kCols = 16;  // (32 at a time spilled registers)
-// The epilogue of 16 accumulator columns (rows c0 .. of the tile) for the lane's output column m.
-// FULL: all 16 rows exist.  Each optional operand is one guarded loop, not a test per element.
+// The epilogue of kCols rows (n of them exist, all if FULL) of output column m, from row `row` of the output on: v holds the
+// sums.  Each optional operand is one guarded loop, not a test per element.
+template <typename TO, bool FULL>
+__device__ __forceinline__ void load_residual(const MmArgs& a, int64_t row, int m, int n, TO (&res)[kCols]) {
+  const TO* r = (const TO*)a.r + row * a.ldr + m;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c, r += a.ldr)
+    if (FULL || c < n) res[c] = *r;
+}
 template <typename TO, int ACT, bool FULL>
-__device__ __forceinline__ void finish_columns(const MmArgs& a, const Tile& x, int m, int c0, uint32_t tmem, bool in, float bias,
-                                               int64_t out_row0) {
-  const int n = FULL ? kCols : x.rows - c0;
-  const int64_t row = out_row0 + c0;
-  TO res[kCols];
-  if (a.r && in) {  // asked for before the accumulators are waited on
-    const TO* r = (const TO*)a.r + row * a.ldr + m;
+__device__ __forceinline__ void finish_values(const MmArgs& a, int64_t row, int m, int n, float bias, const TO (&res)[kCols],
+                                              float (&v)[kCols]) {
 #pragma unroll
-    for (int c = 0; c < kCols; ++c, r += a.ldr)
-      if (FULL || c < n) res[c] = *r;
-  }
-  uint32_t acc[kCols];
-  tmem_ld16(tmem + (uint32_t)c0, acc);
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  if (!in) return;
-  float v[kCols];
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) v[c] = __uint_as_float(acc[c]) + bias;
-  if (x.klen == 0) {  // an empty sum: no MMA wrote the accumulators
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) v[c] = bias;
-  }
+  for (int c = 0; c < kCols; ++c) v[c] += bias;
   if (a.z) {
     TO* z = (TO*)a.z + row * a.ldz + m;
 #pragma unroll
@@ -291,6 +323,22 @@ __device__ __forceinline__ void finish_columns(const MmArgs& a, const Tile& x, i
 #pragma unroll
   for (int c = 0; c < kCols; ++c, y += a.ldy)
     if (FULL || c < n) *y = Wide<TO>::down(v[c]);
+}
+template <typename TO, int ACT, bool FULL>
+__device__ __forceinline__ void finish_columns(const MmArgs& a, const Tile& x, int m, int c0, uint32_t tmem, bool in, float bias,
+                                               int64_t out_row0) {
+  const int n = FULL ? kCols : x.rows - c0;
+  const int64_t row = out_row0 + c0;
+  TO res[kCols];
+  if (a.r && in) load_residual<TO, FULL>(a, row, m, n, res);  // asked for before the accumulators are waited on
+  uint32_t acc[kCols];
+  tmem_ld16(tmem + (uint32_t)c0, acc);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  if (!in) return;
+  float v[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) v[c] = x.klen == 0 ? 0.f : __uint_as_float(acc[c]);  // an empty sum: no MMA wrote them
+  finish_values<TO, ACT, FULL>(a, row, m, n, bias, res, v);
 }
 template <typename TO, int ACT>
 __device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int m, int half, uint32_t tmem, bool in, float bias,
@@ -348,38 +396,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if constexpr (KIND == kGradW) {
     total = a.segments * mblocks * jblocks;
   } else {
-    // exclusive prefix of the segments' tile counts: three consecutive segments per thread
-    constexpr int kPer = (ALPHASPARSE_MAX_EXPERTS + kMmThreads - 1) / kMmThreads;
-    int cnt[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid * kPer + i;
-      const int n = e < a.segments ? s_off[e + 1] - s_off[e] : 0;
-      cnt[i] = n > 0 ? (n + kTileJ - 1) / kTileJ : 0;
-      sum += cnt[i];
-    }
-    int v = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane == 31) s_warp[warp] = v;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kMmThreads / 32; ++w) {
-      if (w < warp) before += s_warp[w];
-      all += s_warp[w];
-    }
-    int run = before + v - sum;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid * kPer + i;
-      if (e < a.segments) s_tile[e] = run;
-      run += cnt[i];
-    }
-    if (tid == 0) s_tile[a.segments] = all;
+    const int all = segment_tiles<kMmThreads, kTileJ>(s_off, a.segments, s_tile, s_warp);
     total = all * mblocks;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -399,8 +416,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const int m = x.m0 + (int)rank * kTileM;
       const int half = x.width / CG;  // rows of the B operand in this CTA
       const int j = x.row0 + (int)rank * half;
-      const int boxes = KIND == kGradW ? (half + 63) / 64 : (half + a.box_rows - 1) / a.box_rows;
-      const uint32_t bytes = kABytes + (uint32_t)(KIND == kGradW ? boxes * kBoxBytes : boxes * a.box_rows * 128);
+      const int box = KIND == kGradW ? 64 : a.box_rows, boxes = (half + box - 1) / box;
+      const uint32_t bytes = kABytes + (uint32_t)(boxes * box * 128);
       for (int c = 0; c < x.klen; c += kKC) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit))) {
           ok = false;
@@ -410,8 +427,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           const uint32_t sa = base + st * kStage, sb = sa + kABytes;
           // a last chunk that has to be cleared completes on the CTA's own barrier; warp 2 passes it on
           const bool own = KIND == kGradW && x.klen - c < kKC && ((x.klen - c) & 15) != 0;
-          const uint32_t bar = own ? tail + 8 * st : CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st;
-          mbar_arrive_tx(own && CG == 2 ? peer_u32(bar, rank) : bar, bytes);
+          const uint32_t bar = own ? (CG == 2 ? peer_u32(tail + 8 * st, rank) : tail + 8 * st) : CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st;
+          mbar_arrive_tx(bar, bytes);
           if constexpr (KIND == kFwdT) {
             tma_3d<CG>(sa, &map_a, c, m, x.e, bar);
           } else if constexpr (KIND == kFwdN) {
@@ -423,7 +440,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           }
           for (int b = 0; b < boxes; ++b) {
             if constexpr (KIND == kGradW) tma_2d<CG>(sb + b * kBoxBytes, &map_b, j + b * 64, x.k0 + c, bar);
-            else tma_2d<CG>(sb + b * a.box_rows * 128, &map_b, c, j + b * a.box_rows, bar);
+            else tma_2d<CG>(sb + b * box * 128, &map_b, c, j + b * box, bar);
           }
         }
         __syncwarp();
@@ -550,6 +567,250 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if (warp == 1) tmem_free<CG>(tmem, kTmemCols);
 }
 
+// ---- few rows: the weights' bytes are the work ----------------------------------------------------
+// One output tile of 128 columns x up to J rows per CLUSTER, whose CTAs share the contraction: each streams its
+// part of K through a ring of its own (several CTAs per SM, so that many loads are in flight),
+// leaves its fp32 sums in shared memory, and after a cluster barrier CTA r adds up the rows r, r + size, ... over all
+// CTAs in rank order (through distributed shared memory) and finishes them.  No workspace, no atomics.
+constexpr int kFewThreads = 192;
+constexpr int kFewStages = 4;
+constexpr int kFewBox = 16;                                  // rows of X per TMA box
+template <int J> struct Few {
+  static constexpr int kStage = kABytes + J * kKC * 2;
+  static constexpr int kSmem = 1024 + kFewStages * kStage + 8 * (2 * kFewStages + 1) + 8;
+  static_assert(kFewStages * kStage >= J * kTileM * 4, "the sums take the ring's place");
+};
+constexpr int kFewTmem = 64;
+
+// Row tile j (of at most J rows) over all segments: false if there are fewer tiles.  Whole warp, without shared memory: a lane counts
+// the tiles of consecutive segments, the lanes' sums are scanned, and the lane that holds tile j finds its segment.
+template <int J>
+__device__ __forceinline__ bool few_tile(int j, const MmArgs& a, Tile& x) {
+  const int lane = threadIdx.x & 31;
+  auto at = [&](int e) { return a.off ? clamp_row(a.off, e, a.rows) : (e == 0 ? 0 : a.rows); };
+  const int per = (a.segments + 31) / 32, e0 = lane * per < a.segments ? lane * per : a.segments;
+  const int e1 = e0 + per < a.segments ? e0 + per : a.segments;
+  int sum = 0, prev = at(e0);
+#pragma unroll 4
+  for (int e = e0; e < e1; ++e) {
+    const int next = at(e + 1);
+    sum += next > prev ? (next - prev + J - 1) / J : 0;
+    prev = next;
+  }
+  int incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  int found = -1, lo = 0, n = 0, k = 0;
+  const bool mine = incl - sum <= j && j < incl;
+  if (mine) {
+    k = j - (incl - sum);
+    prev = at(e0);
+    for (int e = e0; e < e1 && found < 0; ++e) {
+      const int next = at(e + 1), tiles = next > prev ? (next - prev + J - 1) / J : 0;
+      if (k < tiles) {
+        found = e;
+        lo = prev;
+        n = next - prev;
+      } else {
+        k -= tiles;
+        prev = next;
+      }
+    }
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, mine);
+  if (who == 0) return false;
+  const int src = __ffs(who) - 1;
+  x.e = __shfl_sync(0xffffffffu, found, src);
+  lo = __shfl_sync(0xffffffffu, lo, src);
+  n = __shfl_sync(0xffffffffu, n, src);
+  k = __shfl_sync(0xffffffffu, k, src);
+  x.row0 = lo + k * J;
+  x.rows = n - k * J < J ? n - k * J : J;
+  x.width = (x.rows + 15) & ~15;
+  return true;
+}
+
+__device__ __forceinline__ float ld_peer(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename TO, int ACT>
+__device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, int m, int col, uint32_t sums, uint32_t rank, uint32_t size,
+                                              bool in, float bias) {
+  // four rows at a time, their partial sums of all CTAs in flight together
+  for (int j0 = (int)rank; j0 < x.rows; j0 += (int)size * 4) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 0.f;
+    TO res[4];
+    if (!in) continue;
+    if (a.r) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + i * (int)size;
+        if (j < x.rows) res[i] = ((const TO*)a.r)[(int64_t)(x.row0 + j) * a.ldr + m];
+      }
+    }
+    for (uint32_t c = 0; c < size; ++c) {
+      const uint32_t from = peer_u32(sums, c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + i * (int)size;
+        if (j < x.rows) v[i] += ld_peer(from + (uint32_t)(j * kTileM + col) * 4u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i * (int)size;
+      if (j >= x.rows) continue;
+      const int64_t row = x.row0 + j;
+      float w = v[i] + bias;
+      if (a.z) ((TO*)a.z)[row * a.ldz + m] = Wide<TO>::down(w);
+      w = activate<ACT>(w);
+      if (a.r) w += Wide<TO>::up(res[i]);
+      ((TO*)a.y)[row * a.ldy + m] = Wide<TO>::down(w);
+    }
+  }
+}
+
+template <int KIND, int J, typename TO>
+__global__ void __launch_bounds__(kFewThreads)
+expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ MmArgs a,
+                     int size) {
+  constexpr int kStage = Few<J>::kStage;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char* gen = smem_raw + (base - raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gen + kFewStages * kStage);
+  const uint32_t full = base + kFewStages * kStage, empty = full + 8 * kFewStages, acc_full = empty + 8 * kFewStages;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kFewStages + 1);
+  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = size > 1 ? cluster_rank() : 0u;
+  const int mblocks = (a.m_total + kTileM - 1) / kTileM, t = (int)blockIdx.x / size;
+  Tile x;
+  if (!few_tile<J>(t / mblocks, a, x)) return;  // the whole cluster: the grid covers the most tiles these sizes can have
+  x.m0 = (t % mblocks) * kTileM;
+  if (tid == 0) {
+    for (int i = 0; i < kFewStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    mbar_init(acc_full, 1);
+    *s_fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc<1>(smem_u32(s_tmem), kFewTmem);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *s_tmem;
+  const int chunks = (a.k + kKC - 1) / kKC;
+  const int c0 = (int)((int64_t)chunks * rank / size), c1 = (int)((int64_t)chunks * (rank + 1) / size);
+  bool ok = true;
+  if (warp == 0) {
+    const int boxes = x.width / kFewBox;
+    const uint32_t bytes = kABytes + (uint32_t)(boxes * kFewBox * 128);
+    int st = 0;
+    uint32_t ph = 0;
+    for (int c = c0; c < c1; ++c) {
+      if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit))) {
+        ok = false;
+        break;
+      }
+      if (elect_one()) {
+        const uint32_t sa = base + st * kStage, sb = sa + kABytes, bar = full + 8 * st;
+        mbar_arrive_tx(bar, bytes);
+        if constexpr (KIND == kFwdT) {
+          tma_3d<1>(sa, &map_a, c * kKC, x.m0, x.e, bar);
+        } else {
+          tma_3d<1>(sa, &map_a, x.m0, c * kKC, x.e, bar);
+          tma_3d<1>(sa + kBoxBytes, &map_a, x.m0 + 64, c * kKC, x.e, bar);
+        }
+        for (int b = 0; b < boxes; ++b) tma_2d<1>(sb + b * kFewBox * 128, &map_b, c * kKC, x.row0 + b * kFewBox, bar);
+      }
+      __syncwarp();
+      if (++st == kFewStages) {
+        st = 0;
+        ph ^= 1u;
+      }
+    }
+  } else if (warp == 1) {
+    int st = 0;
+    uint32_t ph = 0;
+    constexpr uint32_t kMajor = KIND == kFwdN ? (1u << 15) : 0u;
+    const uint32_t idesc = (1u << 4) | a.types | kMajor | ((uint32_t)(x.width >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+    constexpr uint32_t kStepA = KIND == kFwdT ? 2u : 128u;
+    for (int c = c0; c < c1; ++c) {
+      if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, a.limit))) {
+        ok = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (elect_one()) {
+        const uint64_t da = umma_desc(base + st * kStage, kBoxBytes), db = umma_desc(base + st * kStage + kABytes, kBoxBytes);
+        const int left = a.k - c * kKC, steps = left >= kKC ? kKC / 16 : (left + 15) / 16;
+        for (int s = 0; s < steps; ++s) umma<1>(tmem, da + s * kStepA, db + s * 2u, idesc, c > c0 || s > 0 ? 1u : 0u);
+        umma_commit<1>(empty + 8 * st);
+      }
+      __syncwarp();
+      if (++st == kFewStages) {
+        st = 0;
+        ph ^= 1u;
+      }
+    }
+    if (ok && elect_one()) umma_commit<1>(acc_full);
+    __syncwarp();
+  }
+  const int quarter = warp & 3;
+  const int col = quarter * 32 + lane, m = x.m0 + col;
+  const bool epilogue = warp >= 2, in = epilogue && m < a.m_total;
+  float bias = 0.f;
+  if (epilogue) {
+    if (a.bias && in) bias = load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type);
+    ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0u, a.limit));
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (ok) {
+      // every MMA of this CTA is done: the ring's memory takes the sums, [row][column]
+      float* sums = reinterpret_cast<float*>(gen);
+      for (int j0 = 0; j0 < x.rows; j0 += kCols) {
+        uint32_t acc[kCols];
+        tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)j0, acc);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          if (j0 + c < x.rows) sums[(j0 + c) * kTileM + col] = c0 < c1 ? __uint_as_float(acc[c]) : 0.f;
+      }
+    }
+  }
+  __syncwarp();
+  if (!ok && lane == 0) *s_fail = 1;
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*s_fail) {
+    if (tid == 0) *a.err = 1;
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  if (size > 1) cluster_sync();  // the peers' sums are complete
+  if (epilogue && !*s_fail) {
+    switch (a.act) {
+      case ALPHASPARSE_ACT_RELU: finish_shared<TO, ALPHASPARSE_ACT_RELU>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
+      case ALPHASPARSE_ACT_GELU: finish_shared<TO, ALPHASPARSE_ACT_GELU>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
+      case ALPHASPARSE_ACT_SILU: finish_shared<TO, ALPHASPARSE_ACT_SILU>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
+      default: finish_shared<TO, ALPHASPARSE_ACT_NONE>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1) tmem_free<1>(tmem, kFewTmem);
+  if (size > 1) cluster_sync();  // no CTA leaves while a peer reads its sums
+}
+
 // ---- operands the TMA cannot take: aligned copies -----------------------------------------------
 __global__ void __launch_bounds__(256)
 expert_repack_kernel(const uint16_t* __restrict__ in, int64_t ld, uint16_t* __restrict__ out, int64_t ldo, int64_t rows, int cols) {
@@ -622,13 +883,25 @@ alphasparseStatus_t tensor_map(CUtensorMap* map, const Operand& o, int64_t block
 
 uint32_t type_bits(alphasparseDataType t) { return t == ALPHA_R_16BF ? (1u << 7) | (1u << 10) : 0u; }
 
+// The most shared memory a kernel may take, set once per device.
+template <typename K>
+alphasparseStatus_t allow_smem(K* kernel, int bytes, int device, std::atomic<uint64_t>* done) {
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (device < 64 && (done->load(std::memory_order_relaxed) & bit)) return ALPHA_SPARSE_STATUS_SUCCESS;
+  ASP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done->fetch_or(bit, std::memory_order_relaxed);
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+
 template <int KIND, int CG, typename TO>
 alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles) {
   constexpr int stages = CG == 2 ? kMmStages : 4;
   constexpr size_t smem = 1024 + (size_t)stages * (kABytes + kTileJ / CG * kKC * 2) + 8 * (3 * stages + 4) + 8 +
                           8 * (ALPHASPARSE_MAX_EXPERTS + 1);
-  auto kernel = expert_mm_kernel<KIND, CG, TO>;
-  ASP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> done{0};
+  const auto kernel = expert_mm_kernel<KIND, CG, TO>;
+  const alphasparseStatus_t s = allow_smem(kernel, (int)smem, h->device, &done);
+  if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   const int64_t most = impl(h)->sm_count / CG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
@@ -655,11 +928,56 @@ alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, cons
   }
 }
 
+template <int KIND, int J, typename TO>
+alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles) {
+  static std::atomic<uint64_t> done{0};
+  const auto kernel = expert_mm_few_kernel<KIND, J, TO>;
+  const alphasparseStatus_t s = allow_smem(kernel, Few<J>::kSmem, h->device, &done);
+  if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  // CTAs that share a tile's contraction: as many as fit the device at once, a ring's worth of stages each
+  const int chunks = (a.k + kKC - 1) / kKC, resident = (J == 16 ? 3 : 2) * impl(h)->sm_count;
+  int size = 1;
+  while (size < 8 && tiles * size * 2 <= resident && chunks >= 2 * size * kFewStages) size *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * size));
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = Few<J>::kSmem;
+  cfg.stream = h->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = size > 1 ? 1 : 0;
+  ASP_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, a, size));
+  ++impl(h)->launches;
+  return ALPHA_SPARSE_STATUS_SUCCESS;
+}
+template <int KIND, int J>
+alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
+                               alphasparseDataType out) {
+  switch (out) {
+    case ALPHA_R_32F: return launch_few<KIND, J, float>(h, ma, mb, a, tiles);
+    case ALPHA_R_16F: return launch_few<KIND, J, __half>(h, ma, mb, a, tiles);
+    default: return launch_few<KIND, J, __nv_bfloat16>(h, ma, mb, a, tiles);
+  }
+}
+
 bool type16(alphasparseDataType t) { return t == ALPHA_R_16F || t == ALPHA_R_16BF; }
 
 struct MmShape {
   int64_t rows, n, k;
 };
+// Which kernel: 0 the pair kernel, else the one for few rows per segment with tiles of 16 (1) or 64 rows (2).  Up to 16 rows per
+// segment the weights' bytes are the work and many small CTAs draw them faster (64 experts x 2,048 x 1,408, 64 to 1,024 rows: 74-76 us
+// against 85-87; at 2,048 rows 89 against 87).  Beyond, up to 256 rows, it is the number of pair tiles that decides: a third of the
+// SMs' pairs or less leave the HBM idle (one 4,096 x 4,096 layer, 32 / 128 / 256 rows: 15 / 18 / 24 us against 26 / 28 / 29; 512 rows
+// 35 against 30; eight 2,048 x 2,048 layers, 256 rows: 23 against 22).
+int few_rows(alphasparseHandle_t h, const MmShape& s, int64_t filled) {
+  const int64_t pairs = (s.rows / kTileJ + filled) * ((s.n + 2 * kTileM - 1) / (2 * kTileM));
+  if (s.rows <= 16 * filled) return 1;
+  return s.rows <= 256 * filled && pairs * 3 <= impl(h)->sm_count ? 2 : 0;
+}
 alphasparseStatus_t check_mm(alphasparseHandle_t h, alphasparseOperation_t op, int64_t segments, const int32_t* off,
                              alphasparseDnMatDescr_t x, alphasparseDnMatDescr_t w, alphasparseDnMatDescr_t y, MmShape* shape) {
   if (!h) return ALPHA_SPARSE_STATUS_INVALID_HANDLE;
@@ -744,7 +1062,11 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   a.rows = (int)shape.rows;
   a.m_total = (int)shape.n;
   a.k = (int)shape.k;
-  a.box_rows = 64;
+  // at most: every segment with rows ends in a tile of its own
+  const int64_t filled = segments < shape.rows ? segments : shape.rows;
+  const int few = few_rows(h, shape, filled);
+  // rows of X per box: whole halves of a tile where segments fill tiles, less where a box would mostly fetch rows of other segments
+  a.box_rows = few ? kFewBox : shape.rows > 256 * filled ? 128 : shape.rows > 64 * filled ? 64 : 32;
   a.types = type_bits(x->data_type);
   a.y = y->values;
   a.ldy = y->ld;
@@ -759,8 +1081,13 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
     if ((s = tensor_map(&mw, ow, segments, 64, nk ? kTileM : kKC)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     if ((s = tensor_map(&mx, ox, 0, kKC, (uint32_t)a.box_rows)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   }
-  // at most: every segment with rows ends in a tile of its own
-  const int64_t filled = segments < shape.rows ? segments : shape.rows;
+  if (few) {
+    const int j = few == 1 ? 16 : 64;
+    const int64_t tiles = (shape.rows / j + filled) * ((shape.n + kTileM - 1) / kTileM);
+    if (few == 1)
+      return nk ? launch_few<kFwdT, 16>(h, mw, mx, a, tiles, y->data_type) : launch_few<kFwdN, 16>(h, mw, mx, a, tiles, y->data_type);
+    return nk ? launch_few<kFwdT, 64>(h, mw, mx, a, tiles, y->data_type) : launch_few<kFwdN, 64>(h, mw, mx, a, tiles, y->data_type);
+  }
   const int64_t tiles = (shape.rows / kTileJ + filled) * ((shape.n + 2 * kTileM - 1) / (2 * kTileM));
   return nk ? launch_mm<kFwdT, 2>(h, mw, mx, a, tiles, y->data_type) : launch_mm<kFwdN, 2>(h, mw, mx, a, tiles, y->data_type);
 }

@@ -19,81 +19,117 @@ namespace cg = cooperative_groups;
 namespace asp {
 namespace {
 
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortCluster = 8;             // CTAs of the one-launch sort (portable cluster size)
-// Slots above which the sort runs on the whole device in three launches instead of one cluster.
-constexpr int64_t kSortClusterSlots = 1 << 18;
+constexpr int kSortWarps = 16;
+constexpr int kSortThreads = kSortWarps * 32;
+constexpr int kSortCluster = 8;                  // CTAs of the one-launch sort (portable cluster size)
+constexpr int kSortBatch = 4;                    // ids a lane asks for at a time
+// Slots above which the sort runs on the whole device in two launches instead of one cluster: at 16,384 the cluster's CTAs hold four
+// steps a warp (5.3 us); at 65,536 it would take 10.4 us.
+constexpr int64_t kSortClusterSlots = 1 << 14;
 
+// Shared memory of a sorting CTA: counts[experts][kSortRow] (a column per warp; the odd stride keeps a row's and a column's
+// accesses off the same banks), then totals, all and base[experts], then a word per warp.
+constexpr int kSortRow = kSortWarps + 1;
+constexpr int sort_words(int experts) { return experts * kSortRow + 3 * experts + kSortWarps; }
+
+// The slots of a warp, a multiple of 32 from `begin` on.  Warps and CTAs take ascending ranges, so that counting by CTA, then warp and
+// slot is the stable order.
 struct SlotRange {
-  int begin, end;
+  int64_t begin, end;
 };
-// Warps own contiguous, ascending slot ranges (multiples of 32 slots), so that counting in warp
-// order and then in lane order is the stable order.
-__device__ __forceinline__ SlotRange warp_slots(int slots, int part, int parts) {
-  const int64_t per = ((int64_t)slots + (int64_t)parts * 32 - 1) / ((int64_t)parts * 32) * 32;
-  const int64_t b = per * part, e = b + per;
-  return {(int)(b < slots ? b : slots), (int)(e < slots ? e : slots)};
+__device__ __forceinline__ SlotRange warp_slots(int64_t slots) {
+  const int64_t parts = (int64_t)gridDim.x * kSortWarps, part = (int64_t)blockIdx.x * kSortWarps + (threadIdx.x >> 5);
+  const int64_t per = (slots + parts * 32 - 1) / (parts * 32) * 32, begin = per * part;
+  return {begin, begin + per < slots ? begin + per : slots};
 }
 template <typename Id>
-__device__ __forceinline__ int expert_of(const Id* __restrict__ ids, int slot, int experts) {
-  const Id v = ids[slot];
-  return v >= 0 && v < (Id)experts ? (int)v : -1;
-}
-
-// counts[w][e] of this CTA's warps, then its exclusive prefix over the warps; totals[e] of the CTA.
-template <typename Id>
-__device__ void count_slots(const Id* __restrict__ ids, int slots, int experts, int part0, int parts, int* counts,
-                            int* totals) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int i = tid; i < kSortWarps * experts; i += kSortThreads) counts[i] = 0;
-  __syncthreads();
-  const SlotRange r = warp_slots(slots, part0 + warp, parts);
-  int* mine = counts + warp * experts;
-  for (int s = r.begin + lane; s < r.end; s += 32) {
-    const int e = expert_of(ids, s, experts);
-    if (e >= 0) atomicAdd(&mine[e], 1);  // whole numbers: the order does not matter
-  }
-  __syncthreads();
-  for (int e = tid; e < experts; e += kSortThreads) {
-    int sum = 0;
+__device__ __forceinline__ void load_ids(const Id* __restrict__ ids, int64_t s, int64_t end, int experts, int (&id)[kSortBatch]) {
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = counts[w * experts + e];
-      counts[w * experts + e] = sum;
-      sum += c;
+  for (int i = 0; i < kSortBatch; ++i) {
+    id[i] = -1;
+    if (s + 32 * i < end) {
+      const Id v = ids[s + 32 * i];
+      if (v >= 0 && v < (Id)experts) id[i] = (int)v;
     }
-    totals[e] = sum;
+  }
+}
+
+// counts[e][w]: the slots of e that the CTA's warps before w hold.  totals[e]: the CTA's.
+template <typename Id>
+__device__ __forceinline__ void count_slots(const Id* __restrict__ ids, int experts, SlotRange r, int* counts, int* totals) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int id[kSortBatch];
+  load_ids(ids, r.begin + lane, r.end, experts, id);  // on their way while the counts are cleared
+  for (int i = tid; i < experts * kSortRow; i += kSortThreads) counts[i] = 0;
+  __syncthreads();
+  for (int64_t s = r.begin + lane;;) {
+#pragma unroll
+    for (int i = 0; i < kSortBatch; ++i)
+      if (id[i] >= 0) atomicAdd(&counts[id[i] * kSortRow + warp], 1);  // whole numbers: the order does not matter
+    s += 32 * kSortBatch;
+    if (s - lane >= r.end) break;
+    load_ids(ids, s, r.end, experts, id);
+  }
+  __syncthreads();
+  const int sub = lane % kSortWarps;
+  for (int e0 = warp * 2; e0 < experts; e0 += kSortWarps * 2) {  // half a warp per expert
+    const int e = e0 + lane / kSortWarps;
+    const int c = e < experts ? counts[e * kSortRow + sub] : 0;
+    int v = c;
+#pragma unroll
+    for (int o = 1; o < kSortWarps; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (sub >= o) v += u;
+    }
+    if (e < experts) {
+      counts[e * kSortRow + sub] = v - c;
+      if (sub == kSortWarps - 1) totals[e] = v;
+    }
   }
   __syncthreads();
 }
 
-// position[] of this CTA's slots; counts[w][e] already holds where warp w's first slot of e goes.
-template <typename Id>
-__device__ void place_slots(const Id* __restrict__ ids, int slots, int experts, int part0, int parts, int* counts,
-                            int32_t* __restrict__ position) {
+// position[] of the warp's slots: base[e] is where the CTA's first slot of e goes.
+template <typename Id, int BITS>
+__device__ __forceinline__ void place_slots(const Id* __restrict__ ids, int experts, SlotRange r, int* counts, const int* base,
+                                            int32_t* __restrict__ position) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const SlotRange r = warp_slots(slots, part0 + warp, parts);
-  int* mine = counts + warp * experts;
-  for (int s0 = r.begin; s0 < r.end; s0 += 32) {
-    const int s = s0 + lane;
-    const int e = s < r.end ? expert_of(ids, s, experts) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int before = __popc(same & ((1u << lane) - 1u));
-    const int base = e >= 0 ? mine[e] : 0;
-    __syncwarp();
-    if (e >= 0 && before == 0) mine[e] = base + __popc(same);
-    __syncwarp();
-    if (s < r.end) position[s] = e >= 0 ? base + before : -1;
+  for (int64_t s = r.begin + lane; s - lane < r.end; s += 32 * kSortBatch) {
+    int id[kSortBatch];
+    load_ids(ids, s, r.end, experts, id);
+#pragma unroll
+    for (int i = 0; i < kSortBatch; ++i) {
+      if (s - lane + 32 * i >= r.end) break;
+      const int e = id[i];
+      // lanes with the same expert: a ballot per bit of the number
+      unsigned same = __ballot_sync(0xffffffffu, e >= 0);
+#pragma unroll
+      for (int b = 0; b < BITS; ++b) {
+        const bool bit = (e & (1 << b)) != 0;
+        same &= __ballot_sync(0xffffffffu, bit) ^ (bit ? 0u : ~0u);
+      }
+      const int before = __popc(same & ((1u << lane) - 1u));
+      int* count = &counts[(e >= 0 ? e : 0) * kSortRow + warp];
+      const int at = *count;  // the warp's own column
+      __syncwarp();
+      if (e >= 0 && before == 0) *count = at + __popc(same);
+      __syncwarp();
+      if (s + 32 * i < r.end) position[s + 32 * i] = e >= 0 ? base[e] + at + before : -1;
+    }
   }
 }
 
-// Exclusive prefix over the experts of all[e] (experts <= 2 * kSortThreads), in place; returns the sum.
+// Exclusive prefix over the experts of all[e], in place, consecutive experts per thread; returns the sum.
 __device__ int scan_experts(int* all, int experts, int* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int i0 = 2 * tid, i1 = 2 * tid + 1;
-  const int a = i0 < experts ? all[i0] : 0, b = i1 < experts ? all[i1] : 0;
-  int v = a + b;
+  constexpr int kPer = (ALPHASPARSE_MAX_EXPERTS + kSortThreads - 1) / kSortThreads;
+  int n[kPer], mine = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    n[i] = tid * kPer + i < experts ? all[tid * kPer + i] : 0;
+    mine += n[i];
+  }
+  int v = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -108,102 +144,104 @@ __device__ int scan_experts(int* all, int experts, int* warp_sums) {
     if (w < warp) before += s;
     sum += s;
   }
-  const int excl = before + v - (a + b);
-  if (i0 < experts) all[i0] = excl;
-  if (i1 < experts) all[i1] = excl + a;
+  int run = before + v - mine;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (tid * kPer + i < experts) all[tid * kPer + i] = run;
+    run += n[i];
+  }
   __syncthreads();
   return sum;
 }
-static_assert(ALPHASPARSE_MAX_EXPERTS <= 2 * kSortThreads, "scan_experts holds two experts per thread");
-
 // The whole sort in one launch of one thread-block cluster: counts meet in distributed shared memory.
-// Shared: counts[warps][experts], totals[experts], all[experts], warp_sums[warps].
-template <typename Id>
+template <typename Id, int BITS>
 __global__ void __launch_bounds__(kSortThreads)
-route_sort_cluster_kernel(const Id* __restrict__ ids, int slots, int experts, int32_t* __restrict__ offsets,
+route_sort_cluster_kernel(const Id* __restrict__ ids, int64_t slots, int experts, int32_t* __restrict__ offsets,
                           int32_t* __restrict__ position) {
   extern __shared__ int sort_smem[];
   int* counts = sort_smem;
-  int* totals = counts + kSortWarps * experts;
+  int* totals = counts + experts * kSortRow;
   int* all = totals + experts;
-  int* warp_sums = all + experts;
+  int* base = all + experts;
+  int* warp_sums = base + experts;
   cg::cluster_group cl = cg::this_cluster();
-  const int rank = (int)cl.block_rank(), size = (int)cl.num_blocks();
-  count_slots(ids, slots, experts, rank * kSortWarps, size * kSortWarps, counts, totals);
-  cl.sync();
-  int before[2] = {0, 0};
+  const int size = (int)gridDim.x, cta = (int)blockIdx.x;  // the grid is one cluster
+  const SlotRange r = warp_slots(slots);
+  count_slots(ids, experts, r, counts, totals);
+  if (size > 1) cl.sync();
+  for (int e = threadIdx.x; e < experts; e += kSortThreads) {
+    int sum = totals[e], before = 0;
+    if (size > 1) {
+      int n[kSortCluster];  // (all peers' totals asked for at once)
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = (int)threadIdx.x + i * kSortThreads;
-    if (e < experts) {
-      int sum = 0;
-      for (int c = 0; c < size; ++c) {
-        const int n = *cl.map_shared_rank(totals + e, c);
-        if (c < rank) before[i] += n;
-        sum += n;
+      for (int c = 0; c < kSortCluster; ++c) n[c] = c < size ? *cl.map_shared_rank(totals + e, c) : 0;
+      sum = 0;
+#pragma unroll
+      for (int c = 0; c < kSortCluster; ++c) {
+        if (c < cta) before += n[c];
+        sum += n[c];
       }
-      all[e] = sum;
     }
+    all[e] = sum;
+    base[e] = before;
   }
-  cl.sync();  // every CTA has read its peers' totals: none may leave before, and all[] is complete
+  if (size > 1) cl.sync();  // every CTA has read its peers' totals: none may leave before
+  else __syncthreads();
   const int kept = scan_experts(all, experts, warp_sums);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = (int)threadIdx.x + i * kSortThreads;
-    if (e < experts) {
-      if (rank == 0) offsets[e] = all[e];
-      const int base = all[e] + before[i];
-#pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) counts[w * experts + e] += base;
-    }
+  for (int e = threadIdx.x; e < experts; e += kSortThreads) {
+    if (cta == 0) offsets[e] = all[e];
+    base[e] += all[e];
   }
-  if (rank == 0 && threadIdx.x == 0) offsets[experts] = kept;
+  if (cta == 0 && threadIdx.x == 0) offsets[experts] = kept;
   __syncthreads();
-  place_slots(ids, slots, experts, rank * kSortWarps, size * kSortWarps, counts, position);
+  place_slots<Id, BITS>(ids, experts, r, counts, base, position);
 }
 
-// The same in three launches for long inputs: CTA totals, their prefix over the CTAs and the experts, places.
-template <typename Id, bool PLACE>
+// The same on the whole device in two launches, for long inputs: the CTAs' totals before[b][e]; then every CTA adds them up for itself,
+// those of the CTAs before it and all of them, and places its slots.
+template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
-route_sort_pass_kernel(const Id* __restrict__ ids, int slots, int experts, int* __restrict__ block_base,
-                       int32_t* __restrict__ position) {
+route_sort_count_kernel(const Id* __restrict__ ids, int64_t slots, int experts, int* __restrict__ before) {
+  extern __shared__ int sort_smem[];
+  int* totals = sort_smem + experts * kSortRow;
+  count_slots(ids, experts, warp_slots(slots), sort_smem, totals);
+  for (int e = threadIdx.x; e < experts; e += kSortThreads) before[(size_t)blockIdx.x * experts + e] = totals[e];
+}
+template <typename Id, int BITS>
+__global__ void __launch_bounds__(kSortThreads)
+route_sort_place_kernel(const Id* __restrict__ ids, int64_t slots, int experts, const int* __restrict__ before,
+                        int32_t* __restrict__ offsets, int32_t* __restrict__ position) {
   extern __shared__ int sort_smem[];
   int* counts = sort_smem;
-  int* totals = counts + kSortWarps * experts;
-  const int part0 = (int)blockIdx.x * kSortWarps, parts = (int)gridDim.x * kSortWarps;
-  count_slots(ids, slots, experts, part0, parts, counts, totals);
-  int* base = block_base + (size_t)blockIdx.x * experts;
-  if constexpr (!PLACE) {
-    for (int e = threadIdx.x; e < experts; e += kSortThreads) base[e] = totals[e];
-  } else {
-    for (int i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) counts[i] += base[i % experts];
-    __syncthreads();
-    place_slots(ids, slots, experts, part0, parts, counts, position);
-  }
-}
-__global__ void __launch_bounds__(kSortThreads)
-route_sort_scan_kernel(int* __restrict__ block_base, int blocks, int experts, int32_t* __restrict__ offsets) {
-  __shared__ int all[ALPHASPARSE_MAX_EXPERTS];
-  __shared__ int warp_sums[kSortWarps];
-  for (int e = threadIdx.x; e < experts; e += kSortThreads) {
-    int sum = 0;
+  int* totals = counts + experts * kSortRow;
+  int* all = totals + experts;
+  int* base = all + experts;
+  int* warp_sums = base + experts;
+  const SlotRange r = warp_slots(slots);
+  for (int e = threadIdx.x; e < experts; e += kSortThreads) all[e] = base[e] = 0;
+  count_slots(ids, experts, r, counts, totals);
+  const int parts = experts < kSortThreads ? kSortThreads / experts : 1, blocks = (int)gridDim.x;
+  for (int i = threadIdx.x; i < parts * experts; i += kSortThreads) {
+    const int e = i % experts;
+    int sum = 0, mine = 0;
 #pragma unroll 8
-    for (int b = 0; b < blocks; ++b) sum += block_base[(size_t)b * experts + e];
-    all[e] = sum;
+    for (int b = i / experts; b < blocks; b += parts) {
+      const int c = before[(size_t)b * experts + e];
+      sum += c;
+      mine += b < (int)blockIdx.x ? c : 0;
+    }
+    atomicAdd(&all[e], sum);
+    atomicAdd(&base[e], mine);
   }
   __syncthreads();
   const int kept = scan_experts(all, experts, warp_sums);
   for (int e = threadIdx.x; e < experts; e += kSortThreads) {
-    int run = all[e];
-    offsets[e] = run;
-#pragma unroll 8
-    for (int b = 0; b < blocks; ++b) {
-      const int c = block_base[(size_t)b * experts + e];
-      block_base[(size_t)b * experts + e] = run;
-      run += c;
-    }
+    if (blockIdx.x == 0) offsets[e] = all[e];
+    base[e] += all[e];
   }
-  if (threadIdx.x == 0) offsets[experts] = kept;
+  if (blockIdx.x == 0 && threadIdx.x == 0) offsets[experts] = kept;
+  __syncthreads();
+  place_slots<Id, BITS>(ids, experts, r, counts, base, position);
 }
 
 // ---- row movement ---------------------------------------------------------------------------
@@ -236,9 +274,12 @@ route_dispatch_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs, 
   }
 }
 
-// A warp takes a token's stretch of 32 * U packs of Y and adds up the sorted rows, J of them in flight.
+// A warp takes a token's stretch of 32 * U packs of Y and adds up the sorted rows, J of them in flight.  Bound by HBM: what counts is how
+// many bytes an SM has on the way and how long the pieces of a row are.  1 KB of four rows per warp and three CTAs per SM: 53 us for
+// 8,192 tokens x 8 rows of 2,048 bf16 with a residual (322 MB: 50 us at 6.4 TB/s); 512 bytes of four rows 59 us, of eight rows 64 us;
+// warps that walk over several stretches 90 us (neighbouring stretches of a row then run at different times).
 template <typename T, int V, int U, int J>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 3)
 route_combine_kernel(const T* __restrict__ ys, int64_t ldys, const float* __restrict__ weights, const T* r, int64_t ldr,
                      T* y, int64_t ldy, const int32_t* __restrict__ position, int tokens, int topk, int packs,
                      int stretches, int ys_rows) {
@@ -267,14 +308,10 @@ route_combine_kernel(const T* __restrict__ ys, int64_t ldys, const float* __rest
     const int n = topk - j0 < 32 ? topk - j0 : 32;
     for (int j = 0; j < n; j += J) {
       Pack<T, V> in[J][U];
-      float w[J];
-      bool kept[J];
 #pragma unroll
       for (int i = 0; i < J; ++i) {
         const int p = __shfl_sync(0xffffffffu, mine, (j + i) & 31);
-        w[i] = __shfl_sync(0xffffffffu, w_mine, (j + i) & 31);
-        kept[i] = j + i < n && (unsigned)p < (unsigned)ys_rows;
-        if (kept[i]) {
+        if (j + i < n && (unsigned)p < (unsigned)ys_rows) {
 #pragma unroll
           for (int u = 0; u < U; ++u)
             if (c0 + 32 * u < packs) in[i][u] = load_pack<T, V>(ys + (int64_t)p * ldys + (int64_t)(c0 + 32 * u) * V);
@@ -282,12 +319,14 @@ route_combine_kernel(const T* __restrict__ ys, int64_t ldys, const float* __rest
       }
 #pragma unroll
       for (int i = 0; i < J; ++i) {
-        if (!kept[i]) continue;
+        const int p = __shfl_sync(0xffffffffu, mine, (j + i) & 31);
+        const float w = __shfl_sync(0xffffffffu, w_mine, (j + i) & 31);
+        if (j + i >= n || (unsigned)p >= (unsigned)ys_rows) continue;
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (c0 + 32 * u < packs) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[u][v] = fmaf(w[i], Wide<T>::up(in[i][u].v[v]), acc[u][v]);
+            for (int v = 0; v < V; ++v) acc[u][v] = fmaf(w, in[i][u].at(v), acc[u][v]);
           }
       }
     }
@@ -297,17 +336,39 @@ route_combine_kernel(const T* __restrict__ ys, int64_t ldys, const float* __rest
     if (c0 + 32 * u < packs) {
       if (r) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[u][v] += Wide<T>::up(res[u].v[v]);
+        for (int v = 0; v < V; ++v) acc[u][v] += res[u].at(v);
       }
       store_pack<T, V>(y + (int64_t)t * ldy + (int64_t)(c0 + 32 * u) * V, round_pack<T, V>(acc[u]));
     }
 }
 
-// Gradient of combine.  blockDim.y tokens per CTA, blockDim.x threads on a token's row (whole warps).
-// The dot products of J slots are kept at a time and added up over lanes, then over the row's warps,
-// in a fixed order.
+// Sums of J values over the lanes of a warp (J a power of two, at most 32): lane l ends with the sum of value l % J.
+// While more than one value is left, each step sends half of them to the partner and adds the half that comes back:
+// 9 shuffles for J = 8 instead of 40.
+template <int J>
+__device__ __forceinline__ float reduce_values(float (&v)[J], int lane) {
+#pragma unroll
+  for (int n = J / 2; n > 0; n /= 2) {
+    const bool up = (lane & n) != 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+    }
+  }
+#pragma unroll
+  for (int o = J; o < 32; o *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+
+// Gradient of combine.  blockDim.y tokens per CTA, blockDim.x threads on a token's row (whole warps).  J slots at a time: their rows
+// of Ys are all asked for before the first is used; their dot products are added up over lanes, then over the row's warps, in a
+// fixed order.  Bound by HBM (435 MB at 8,192 tokens x 6 rows of 2,048 bf16: 68 us at 6.4 TB/s): four rows in flight, two tokens per CTA
+// and four CTAs per SM take 81 us; one token per CTA 90 us; eight rows in flight (three CTAs fit) 105 us, without a register limit
+// (one CTA) 189 us.
+constexpr int kGradThreads = 128;  // of a token
 template <typename T, int V, int J>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 4)
 route_combine_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* ys, int64_t ldys,
                           const float* __restrict__ weights, T* dys, int64_t lddys, float* __restrict__ dweights,
                           const int32_t* __restrict__ position, int tokens, int topk, int packs, int rows) {
@@ -316,47 +377,50 @@ route_combine_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* ys, i
   const int lane = threadIdx.x & 31;
   const int warps = (int)blockDim.x >> 5, row_warp0 = (int)threadIdx.y * warps, my_warp = row_warp0 + ((int)threadIdx.x >> 5);
   for (int j0 = 0; j0 < topk; j0 += J) {
-    int p[J];
-    float w[J], dot[J];
-#pragma unroll
-    for (int i = 0; i < J; ++i) {
-      const bool in = t < tokens && j0 + i < topk;
-      p[i] = in ? position[(int64_t)t * topk + j0 + i] : -1;
-      w[i] = in && weights ? weights[(int64_t)t * topk + j0 + i] : 1.f;
-      dot[i] = 0.f;
+    // lane i of every warp holds slot j0 + i
+    int p_mine = -1;
+    float w_mine = 1.f;
+    if (t < tokens && lane < J && j0 + lane < topk) {
+      p_mine = position[(int64_t)t * topk + j0 + lane];
+      if (weights) w_mine = weights[(int64_t)t * topk + j0 + lane];
     }
+    float dot[J];
+#pragma unroll
+    for (int i = 0; i < J; ++i) dot[i] = 0.f;
     if (t < tokens) {
-      for (int c = (int)threadIdx.x; c < packs; c += (int)blockDim.x) {
-        const Pack<T, V> g = load_pack<T, V>(dy + (int64_t)t * lddy + (int64_t)c * V);
-        Pack<T, V> in[J];
+      // (whole warps step together: the shuffles below need every lane)
+      for (int c0 = (int)threadIdx.x - lane; c0 < packs; c0 += (int)blockDim.x) {
+        const int c = c0 + lane;
+        const bool in_row = c < packs;
+        Pack<T, V> g, in[J];
+        if (in_row) g = load_pack<T, V>(dy + (int64_t)t * lddy + (int64_t)c * V);
         if (dweights) {
 #pragma unroll
-          for (int i = 0; i < J; ++i)
-            if ((unsigned)p[i] < (unsigned)rows) in[i] = load_pack<T, V>(ys + (int64_t)p[i] * ldys + (int64_t)c * V);
+          for (int i = 0; i < J; ++i) {
+            const int p = __shfl_sync(0xffffffffu, p_mine, i);
+            if (in_row && (unsigned)p < (unsigned)rows) in[i] = load_pack<T, V>(ys + (int64_t)p * ldys + (int64_t)c * V);
+          }
         }
 #pragma unroll
         for (int i = 0; i < J; ++i) {
-          if ((unsigned)p[i] >= (unsigned)rows) continue;
+          const int p = __shfl_sync(0xffffffffu, p_mine, i);
+          const float w = __shfl_sync(0xffffffffu, w_mine, i);
+          if (!in_row || (unsigned)p >= (unsigned)rows) continue;
           float out[V];
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float gv = Wide<T>::up(g.v[v]);
-            if (dweights) dot[i] = fmaf(gv, Wide<T>::up(in[i].v[v]), dot[i]);
-            out[v] = w[i] * gv;
+            const float gv = g.at(v);
+            if (dweights) dot[i] = fmaf(gv, in[i].at(v), dot[i]);
+            out[v] = w * gv;
           }
-          if (dys) store_pack<T, V>(dys + (int64_t)p[i] * lddys + (int64_t)c * V, round_pack<T, V>(out));
+          if (dys) store_pack<T, V>(dys + (int64_t)p * lddys + (int64_t)c * V, round_pack<T, V>(out));
         }
+        __syncwarp();
       }
     }
     if (!dweights) continue;
-#pragma unroll
-    for (int i = 0; i < J; ++i)
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], o);
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < J; ++i) part[my_warp][i] = dot[i];
-    }
+    const float sum_mine = reduce_values<J>(dot, lane);
+    if (lane < J) part[my_warp][lane] = sum_mine;
     __syncthreads();
     if (t < tokens && (int)threadIdx.x < J && j0 + (int)threadIdx.x < topk) {
       float sum = 0.f;
@@ -383,19 +447,20 @@ alphasparseStatus_t by_type(alphasparseDataType t, F f) {
   }
 }
 
-int sort_blocks(alphasparseHandle_t h) { return impl(h)->sm_count; }
+// CTAs of the two-launch sort: four steps a warp or more, no more than one per SM.
+int64_t sort_blocks(alphasparseHandle_t h, int64_t slots) { return std::min<int64_t>((slots + 2047) / 2048, impl(h)->sm_count); }
 
-template <typename Id>
+template <typename Id, int BITS>
 alphasparseStatus_t run_sort(alphasparseHandle_t h, alphasparseRoutingDescr_t r, void* buffer) {
-  const int slots = (int)(r->tokens * r->topk), experts = (int)r->experts;
+  const int64_t slots = r->tokens * r->topk;
+  const int experts = (int)r->experts;
   const Id* ids = (const Id*)r->expert_ids;
-  const size_t smem = sizeof(int) * ((size_t)kSortWarps * experts + 2 * (size_t)experts + kSortWarps);
+  const size_t smem = sizeof(int) * (size_t)sort_words(experts);
+  const int most = (int)sizeof(int) * sort_words(ALPHASPARSE_MAX_EXPERTS);
   if (slots <= kSortClusterSlots) {
-    if (smem > 48 * 1024)
-      ASP_CUDA(cudaFuncSetAttribute(route_sort_cluster_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)(sizeof(int) * ((kSortWarps + 2) * ALPHASPARSE_MAX_EXPERTS + kSortWarps))));
-    // a CTA per 2,048 slots (four rounds of its warps' lanes): few slots need no cluster
-    int ctas = 1;
+    const auto kernel = route_sort_cluster_kernel<Id, BITS>;
+    if (smem > 48 * 1024) ASP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    int ctas = 1;  // a CTA per 2,048 slots (four steps of its warps), as far as a cluster goes
     while (ctas < kSortCluster && ctas * 2048 < slots) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
@@ -407,27 +472,31 @@ alphasparseStatus_t run_sort(alphasparseHandle_t h, alphasparseRoutingDescr_t r,
     at[0].val.clusterDim.x = ctas;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
-    ASP_CUDA(cudaLaunchKernelEx(&cfg, route_sort_cluster_kernel<Id>, ids, slots, experts, r->expert_offsets, r->position));
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
+    ASP_CUDA(cudaLaunchKernelEx(&cfg, kernel, ids, slots, experts, r->expert_offsets, r->position));
     ++impl(h)->launches;
     return ALPHA_SPARSE_STATUS_SUCCESS;
   }
-  if (!buffer) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
-  int* base = reinterpret_cast<int*>((reinterpret_cast<uintptr_t>(buffer) + 15) & ~(uintptr_t)15);
-  const int blocks = sort_blocks(h);
-  const int most = (int)(sizeof(int) * (kSortWarps + 2) * ALPHASPARSE_MAX_EXPERTS);
-  ASP_CUDA(cudaFuncSetAttribute(route_sort_pass_kernel<Id, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-  ASP_CUDA(cudaFuncSetAttribute(route_sort_pass_kernel<Id, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-  const size_t pass_smem = sizeof(int) * (size_t)(kSortWarps + 1) * experts;
-  route_sort_pass_kernel<Id, false><<<blocks, kSortThreads, pass_smem, h->stream>>>(ids, slots, experts, base, nullptr);
+  const int blocks = (int)sort_blocks(h, slots);
+  int* before = reinterpret_cast<int*>((reinterpret_cast<uintptr_t>(buffer) + 15) & ~(uintptr_t)15);
+  const auto count = route_sort_count_kernel<Id>;
+  const auto place = route_sort_place_kernel<Id, BITS>;
+  if (smem > 48 * 1024) {
+    ASP_CUDA(cudaFuncSetAttribute(count, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    ASP_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  }
+  count<<<blocks, kSortThreads, smem, h->stream>>>(ids, slots, experts, before);
   ASP_CUDA(cudaGetLastError());
-  route_sort_scan_kernel<<<1, kSortThreads, 0, h->stream>>>(base, blocks, experts, r->expert_offsets);
+  place<<<blocks, kSortThreads, smem, h->stream>>>(ids, slots, experts, before, r->expert_offsets, r->position);
   ASP_CUDA(cudaGetLastError());
-  route_sort_pass_kernel<Id, true><<<blocks, kSortThreads, pass_smem, h->stream>>>(ids, slots, experts, base, r->position);
-  ASP_CUDA(cudaGetLastError());
-  impl(h)->launches += 3;
+  impl(h)->launches += 2;
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
+template <typename Id>
+alphasparseStatus_t run_sort(alphasparseHandle_t h, alphasparseRoutingDescr_t r, void* buffer) {
+  return r->experts <= 64 ? run_sort<Id, 6>(h, r, buffer) : run_sort<Id, 10>(h, r, buffer);
+}
+static_assert(ALPHASPARSE_MAX_EXPERTS <= 1 << 10, "ten ballots tell the experts apart");
 
 // Warps for tokens x stretches, as a grid; 0 when there is nothing to do.
 int64_t row_blocks(int64_t tokens, int64_t stretches) { return (tokens * stretches * 32 + kRowThreads - 1) / kRowThreads; }
@@ -450,7 +519,7 @@ alphasparseStatus_t run_dispatch(alphasparseHandle_t h, alphasparseRoutingDescr_
 template <typename T, int V>
 alphasparseStatus_t run_combine(alphasparseHandle_t h, alphasparseRoutingDescr_t r, alphasparseDnMatDescr_t ys,
                                 const float* weights, alphasparseDnMatDescr_t res, alphasparseDnMatDescr_t y) {
-  constexpr int U = V == 1 ? 4 : 1;
+  constexpr int U = V == 1 ? 8 : 2;
   const int64_t packs = y->cols / V, stretches = (packs + 32 * U - 1) / (32 * U);
   const int64_t blocks = row_blocks(r->tokens, stretches);
   if (blocks >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
@@ -468,10 +537,10 @@ alphasparseStatus_t run_combine_grad(alphasparseHandle_t h, alphasparseRoutingDe
                                      float* dweights, int64_t rows) {
   const int64_t packs = dy->cols / V;
   int x = 32;
-  while (x < kRowThreads && x < packs) x *= 2;
+  while (x < kGradThreads && x < packs) x *= 2;
   const int y = kRowThreads / x;
   const int64_t blocks = (r->tokens + y - 1) / y;
-  route_combine_grad_kernel<T, V, 8><<<(unsigned)blocks, dim3(x, y), 0, h->stream>>>(
+  route_combine_grad_kernel<T, V, 4><<<(unsigned)blocks, dim3(x, y), 0, h->stream>>>(
       (const T*)dy->values, dy->ld, ys ? (const T*)ys->values : nullptr, ys ? ys->ld : 0, weights,
       dys ? (T*)dys->values : nullptr, dys ? dys->ld : 0, dweights, r->position, (int)r->tokens, (int)r->topk, (int)packs,
       (int)rows);
@@ -491,7 +560,7 @@ alphasparseStatus_t alphasparseRoutingSort_bufferSize(alphasparseHandle_t h, alp
   if (!size) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   const alphasparseStatus_t s = check_routing(h, r);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-  *size = r->tokens * r->topk <= kSortClusterSlots ? 0 : sizeof(int) * (size_t)sort_blocks(h) * r->experts + 16;
+  *size = r->tokens * r->topk <= kSortClusterSlots ? 0 : sizeof(int) * (size_t)(sort_blocks(h, r->tokens * r->topk) * r->experts) + 16;
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "asp_internal.h"
 
@@ -25,37 +26,60 @@ template <> struct Wide<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
+// A pack as 32-bit words (16-bit elements stay two to a register until they are used), or one element.
 template <typename T, int V> struct Pack {
-  static_assert(V == 1 || V * sizeof(T) == 16, "a pack is one element or 16 bytes");
-  T v[V];
+  static_assert(V * sizeof(T) == 16, "a pack is one element or 16 bytes");
+  uint32_t w[4];
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
+  }
+};
+template <typename T> struct Pack<T, 1> {
+  T v;
+  __device__ __forceinline__ float at(int) const { return Wide<T>::up(v); }
 };
 
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   Pack<T, V> r;
   if constexpr (V == 1) {
-    r.v[0] = *p;
+    r.v = *p;
   } else {
     const uint4 u = *reinterpret_cast<const uint4*>(p);
-    memcpy(r.v, &u, 16);
+    r.w[0] = u.x;
+    r.w[1] = u.y;
+    r.w[2] = u.z;
+    r.w[3] = u.w;
   }
   return r;
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
-  if constexpr (V == 1) {
-    *p = r.v[0];
-  } else {
-    uint4 u;
-    memcpy(&u, r.v, 16);
-    *reinterpret_cast<uint4*>(p) = u;
-  }
+  if constexpr (V == 1) *p = r.v;
+  else *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
 }
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> round_pack(const float (&f)[V]) {
   Pack<T, V> r;
+  if constexpr (V == 1) {
+    r.v = Wide<T>::down(f[0]);
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = Wide<T>::down(f[i]);
+    for (int i = 0; i < 4; ++i) r.w[i] = __float_as_uint(f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        memcpy(&r.w[i], &h, 4);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        memcpy(&r.w[i], &h, 4);
+      }
+    }
+  }
   return r;
 }
 

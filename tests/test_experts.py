@@ -258,7 +258,8 @@ def test_act_grad_refusals():
 @pytest.mark.parametrize("tokens,topk,experts,dtype", [
     (0, 2, 8, torch.int32), (1, 1, 1, torch.int64), (1, 8, 64, torch.int32), (3, 5, 7, torch.int64), (33, 2, 1024, torch.int32),
     (1000, 3, 61, torch.int64), (4096, 8, 256, torch.int32), (40000, 6, 1000, torch.int64), (70001, 4, 1024, torch.int32),
-    (300007, 1, 3, torch.int64), (9, 64, 70, torch.int32)])
+    (300007, 1, 3, torch.int64), (9, 64, 70, torch.int32),
+    (8192, 2, 64, torch.int32), (16385, 1, 65, torch.int64), (128, 2, 5, torch.int64)])
 def test_sort(h, tokens, topk, experts, dtype):
     g = gen(tokens + topk)
     skew = (torch.rand(tokens, topk, device="cuda", generator=g) ** 2 * (experts + 2)).to(dtype) - 1   # -1 .. experts: both ends drop
@@ -277,7 +278,7 @@ def test_sort(h, tokens, topk, experts, dtype):
 def test_sort_all_slots_alike(h, fill):
     ids = torch.full((20000, 2), fill, dtype=torch.int32, device="cuda")
     r = api.Routing(ids, 6)
-    api.routing_sort(h, r)
+    api.routing_sort(h, r, buffer(api.routing_buffer_size(h, r)))
     off, pos = places(ids, 6)
     assert torch.equal(r.offsets.cpu(), off) and torch.equal(r.position.cpu(), pos)
 
