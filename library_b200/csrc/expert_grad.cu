@@ -7,6 +7,7 @@
 // one that goes on.  A second kernel adds up the pieces of such segments in chunk order and
 // zeroes the rows of empty segments.  No atomics: the sums do not depend on the order of the CTAs.
 #include "expert_act.h"
+#include "expert_launch.h"
 #include "expert_vec.h"
 
 namespace asp {
@@ -33,6 +34,8 @@ expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz
   const int chunk = (int)(blockIdx.x / (unsigned)strips), strip = (int)(blockIdx.x % (unsigned)strips);
   const int r0 = chunk * kActRows, r1 = r0 < rows - kActRows ? r0 + kActRows : rows;
   const int c0 = strip * 32 * V, c = c0 + lane * V;
+  dependency_wait();
+  dependents_go();
   // the last segment that begins at or before the chunk
   int before = 0;
   for (int i = 0; i <= segments; i += kActThreads)
@@ -93,6 +96,8 @@ __global__ void __launch_bounds__(kActThreads)
 expert_bias_join_kernel(float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
                         int cols, int strips, const float* __restrict__ pieces) {
   __shared__ float part[kJoinParts][kJoinCols];
+  dependency_wait();
+  dependents_go();
   const int q = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
   const int e = (int)(blockIdx.x / (unsigned)strips), c = (int)(blockIdx.x % (unsigned)strips) * kJoinCols + i;
   const int b = clamp_row(off, e, segments, rows), d = clamp_row(off, e + 1, segments, rows);
@@ -127,22 +132,17 @@ alphasparseStatus_t run_act_grad(alphasparseHandle_t h, int segments, const int3
   float* pieces = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(buffer) + 15) & ~(uintptr_t)15);
   if (chunks * strips >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
   if (chunks > 0) {
-    expert_act_grad_kernel<T, V, ACT><<<(unsigned)(chunks * strips), kActThreads, 0, h->stream>>>(
-        (const T*)dy->values, dy->ld, z ? (const T*)z->values : nullptr, z ? z->ld : 0, dz ? (T*)dz->values : nullptr,
-        dz ? dz->ld : 0, db ? (float*)db->values : nullptr, db ? db->ld : 0, off, segments, rows, cols, (int)strips,
-        pieces);
-    ASP_CUDA(cudaGetLastError());
-    ++impl(h)->launches;
+    const alphasparseStatus_t s = launch_chained(
+        h, expert_act_grad_kernel<T, V, ACT>, dim3((unsigned)(chunks * strips)), dim3(kActThreads), 0, 1, (const T*)dy->values, dy->ld,
+        z ? (const T*)z->values : nullptr, z ? z->ld : 0, dz ? (T*)dz->values : nullptr, dz ? dz->ld : 0,
+        db ? (float*)db->values : nullptr, db ? db->ld : 0, off, segments, rows, cols, (int)strips, pieces);
+    if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   }
-  if (db) {
-    const int64_t js = ((int64_t)cols + kJoinCols - 1) / kJoinCols;
-    if (segments * js >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
-    expert_bias_join_kernel<<<(unsigned)(segments * js), kActThreads, 0, h->stream>>>(
-        (float*)db->values, db->ld, off, segments, rows, cols, (int)js, pieces);
-    ASP_CUDA(cudaGetLastError());
-    ++impl(h)->launches;
-  }
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+  if (!db) return ALPHA_SPARSE_STATUS_SUCCESS;
+  const int64_t js = ((int64_t)cols + kJoinCols - 1) / kJoinCols;
+  if (segments * js >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  return launch_chained(h, expert_bias_join_kernel, dim3((unsigned)(segments * js)), dim3(kActThreads), 0, 1, (float*)db->values, db->ld,
+                        off, segments, rows, cols, (int)js, (const float*)pieces);
 }
 
 template <typename T>

@@ -12,6 +12,7 @@
 #include <atomic>
 
 #include "expert_act.h"
+#include "expert_launch.h"
 #include "expert_vec.h"
 
 namespace asp {
@@ -69,6 +70,9 @@ __device__ __forceinline__ bool elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(pred));
   return pred != 0;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 // TMA loads into this CTA's shared memory.  The .cta_group::2 form may complete on a barrier of either CTA of the pair.
 template <int CG>
@@ -390,6 +394,13 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc<CG>(smem_u32(s_tmem), kTmemCols);
+  if (tid == 32 * 3) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
+  __syncthreads();
+  dependents_go();  // tensor memory is allocated
+  dependency_wait();
   for (int i = tid; i <= a.segments; i += kMmThreads) s_off[i] = a.off ? clamp_row(a.off, i, a.rows) : (i == 0 ? 0 : a.rows);
   __syncthreads();
   int total;
@@ -693,9 +704,6 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = size > 1 ? cluster_rank() : 0u;
   const int mblocks = (a.m_total + kTileM - 1) / kTileM, t = (int)blockIdx.x / size;
-  Tile x;
-  if (!few_tile<J>(t / mblocks, a, x)) return;  // the whole cluster: the grid covers the most tiles these sizes can have
-  x.m0 = (t % mblocks) * kTileM;
   if (tid == 0) {
     for (int i = 0; i < kFewStages; ++i) {
       mbar_init(full + 8 * i, 1);
@@ -706,10 +714,22 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc<1>(smem_u32(s_tmem), kFewTmem);
+  if (tid == 64) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *s_tmem;
+  dependents_go();  // tensor memory is allocated
+  dependency_wait();
+  Tile x;
+  if (!few_tile<J>(t / mblocks, a, x)) {  // the whole cluster: the grid covers the most tiles these sizes can have
+    if (warp == 1) tmem_free<1>(tmem, kFewTmem);
+    return;
+  }
+  x.m0 = (t % mblocks) * kTileM;
   const int chunks = (a.k + kKC - 1) / kKC;
   const int c0 = (int)((int64_t)chunks * rank / size), c1 = (int)((int64_t)chunks * (rank + 1) / size);
   bool ok = true;
@@ -812,12 +832,34 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 }
 
 // ---- operands the TMA cannot take: aligned copies -----------------------------------------------
+struct Copy16 {
+  const uint16_t* in;
+  uint16_t* out;
+  int64_t rows, ld, ldo;
+  int cols;
+};
+// Up to two matrices in one launch; a warp per row.
 __global__ void __launch_bounds__(256)
-expert_repack_kernel(const uint16_t* __restrict__ in, int64_t ld, uint16_t* __restrict__ out, int64_t ldo, int64_t rows, int cols) {
+expert_repack_kernel(const __grid_constant__ Copy16 a, const __grid_constant__ Copy16 b) {
+  dependency_wait();
+  dependents_go();
   const int lane = threadIdx.x & 31;
-  for (int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; r < rows; r += (int64_t)gridDim.x * 8)
-#pragma unroll 8
-    for (int c = lane; c < cols; c += 32) out[r * ldo + c] = in[r * ld + c];
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; i < a.rows + b.rows; i += (int64_t)gridDim.x * 8) {
+    const Copy16& m = i < a.rows ? a : b;
+    const int64_t r = i < a.rows ? i : i - a.rows;
+    const uint16_t* in = m.in + r * m.ld;
+    uint16_t* out = m.out + r * m.ldo;
+    constexpr int kBatch = 8;  // loads in flight
+    for (int c = lane; c < m.cols; c += 32 * kBatch) {
+      uint16_t v[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (c + 32 * k < m.cols) v[k] = in[c + 32 * k];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (c + 32 * k < m.cols) out[c + 32 * k] = v[k];
+    }
+  }
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -851,18 +893,23 @@ size_t repack_bytes(alphasparseDnMatDescr_t a, alphasparseDnMatDescr_t b) {
   const size_t n = repack_bytes(a) + repack_bytes(b);
   return n ? n + 256 : 0;
 }
-alphasparseStatus_t ready_operand(alphasparseHandle_t h, alphasparseDnMatDescr_t m, unsigned char** scratch, Operand* o) {
-  *o = {m->values, m->rows, m->cols, m->ld, m->data_type};
-  if (tma_ready(m)) return ALPHA_SPARSE_STATUS_SUCCESS;
-  o->p = *scratch;
-  o->ld = padded8(m->cols);
-  *scratch += repack_bytes(m);
-  const int64_t blocks = (m->rows + 7) / 8;
-  expert_repack_kernel<<<(unsigned)(blocks < 8 * impl(h)->sm_count ? blocks : 8 * impl(h)->sm_count), 256, 0, h->stream>>>(
-      (const uint16_t*)m->values, m->ld, (uint16_t*)o->p, o->ld, m->rows, (int)m->cols);
-  ASP_CUDA(cudaGetLastError());
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+alphasparseStatus_t ready_operands(alphasparseHandle_t h, alphasparseDnMatDescr_t ma, alphasparseDnMatDescr_t mb, void* buffer, Operand* a,
+                                   Operand* b) {
+  unsigned char* scratch = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(buffer) + 255) & ~(uintptr_t)255);
+  Copy16 copies[2] = {};
+  alphasparseDnMatDescr_t m[2] = {ma, mb};
+  Operand* o[2] = {a, b};
+  for (int i = 0; i < 2; ++i) {
+    *o[i] = {m[i]->values, m[i]->rows, m[i]->cols, m[i]->ld, m[i]->data_type};
+    if (tma_ready(m[i])) continue;
+    o[i]->p = scratch;
+    o[i]->ld = padded8(m[i]->cols);
+    copies[i] = {(const uint16_t*)m[i]->values, (uint16_t*)o[i]->p, m[i]->rows, m[i]->ld, o[i]->ld, (int)m[i]->cols};
+    scratch += repack_bytes(m[i]);
+  }
+  const int64_t blocks = (copies[0].rows + copies[1].rows + 7) / 8, most = 8 * (int64_t)impl(h)->sm_count;
+  if (blocks == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
+  return launch_chained(h, expert_repack_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, 1, copies[0], copies[1]);
 }
 
 // blocks > 0: a third dimension over stacked blocks of rows / blocks rows each (out-of-range rows of a block read as
@@ -903,20 +950,7 @@ alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, cons
   const alphasparseStatus_t s = allow_smem(kernel, (int)smem, h->device, &done);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   const int64_t most = impl(h)->sm_count / CG;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
-  cfg.blockDim = dim3(kMmThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = h->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  ASP_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, a));
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+  return launch_chained(h, kernel, dim3((unsigned)((tiles < most ? tiles : most) * CG)), dim3(kMmThreads), smem, CG, ma, mb, a);
 }
 template <int KIND, int CG>
 alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
@@ -938,20 +972,7 @@ alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, con
   const int chunks = (a.k + kKC - 1) / kKC, resident = (J == 16 ? 3 : 2) * impl(h)->sm_count;
   int size = 1;
   while (size < 8 && tiles * size * 2 <= resident && chunks >= 2 * size * kFewStages) size *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * size));
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = Few<J>::kSmem;
-  cfg.stream = h->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = size;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = size > 1 ? 1 : 0;
-  ASP_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, a, size));
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+  return launch_chained(h, kernel, dim3((unsigned)(tiles * size)), dim3(kFewThreads), Few<J>::kSmem, size, ma, mb, a, size);
 }
 template <int KIND, int J>
 alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
@@ -1052,10 +1073,8 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
   const bool nk = op == ALPHA_SPARSE_OPERATION_TRANSPOSE;
-  unsigned char* scratch = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(buffer) + 255) & ~(uintptr_t)255);
   Operand ox, ow;
-  if ((s = ready_operand(h, x, &scratch, &ox)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-  if ((s = ready_operand(h, w, &scratch, &ow)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  if ((s = ready_operands(h, x, w, buffer, &ox, &ow)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   MmArgs a = {};
   a.off = off;
   a.segments = (int)segments;
@@ -1114,10 +1133,8 @@ alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparse
   if (!buffer && repack_bytes(x, dz)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
-  unsigned char* scratch = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(buffer) + 255) & ~(uintptr_t)255);
   Operand om, oj;
-  if ((s = ready_operand(h, m, &scratch, &om)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-  if ((s = ready_operand(h, j, &scratch, &oj)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  if ((s = ready_operands(h, m, j, buffer, &om, &oj)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   MmArgs a = {};
   a.off = off;
   a.segments = (int)segments;

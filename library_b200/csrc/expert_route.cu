@@ -12,6 +12,7 @@
 
 #include <algorithm>
 
+#include "expert_launch.h"
 #include "expert_vec.h"
 
 namespace cg = cooperative_groups;
@@ -164,6 +165,8 @@ route_sort_cluster_kernel(const Id* __restrict__ ids, int64_t slots, int experts
   int* all = totals + experts;
   int* base = all + experts;
   int* warp_sums = base + experts;
+  dependency_wait();
+  dependents_go();
   cg::cluster_group cl = cg::this_cluster();
   const int size = (int)gridDim.x, cta = (int)blockIdx.x;  // the grid is one cluster
   const SlotRange r = warp_slots(slots);
@@ -204,6 +207,8 @@ __global__ void __launch_bounds__(kSortThreads)
 route_sort_count_kernel(const Id* __restrict__ ids, int64_t slots, int experts, int* __restrict__ before) {
   extern __shared__ int sort_smem[];
   int* totals = sort_smem + experts * kSortRow;
+  dependency_wait();
+  dependents_go();
   count_slots(ids, experts, warp_slots(slots), sort_smem, totals);
   for (int e = threadIdx.x; e < experts; e += kSortThreads) before[(size_t)blockIdx.x * experts + e] = totals[e];
 }
@@ -219,6 +224,8 @@ route_sort_place_kernel(const Id* __restrict__ ids, int64_t slots, int experts, 
   int* warp_sums = base + experts;
   const SlotRange r = warp_slots(slots);
   for (int e = threadIdx.x; e < experts; e += kSortThreads) all[e] = base[e] = 0;
+  dependency_wait();
+  dependents_go();
   count_slots(ids, experts, r, counts, totals);
   const int parts = experts < kSortThreads ? kSortThreads / experts : 1, blocks = (int)gridDim.x;
   for (int i = threadIdx.x; i < parts * experts; i += kSortThreads) {
@@ -254,6 +261,8 @@ route_dispatch_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs, 
                       const int32_t* __restrict__ position, int tokens, int topk, int packs, int stretches, int xs_rows) {
   const int lane = threadIdx.x & 31;
   const int64_t task = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
+  dependency_wait();
+  dependents_go();
   if (task >= (int64_t)tokens * stretches) return;
   const int t = (int)(task / stretches), c0 = (int)(task % stretches) * (32 * U) + lane;
   Pack<T, V> row[U];
@@ -285,6 +294,8 @@ route_combine_kernel(const T* __restrict__ ys, int64_t ldys, const float* __rest
                      int stretches, int ys_rows) {
   const int lane = threadIdx.x & 31;
   const int64_t task = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
+  dependency_wait();
+  dependents_go();
   if (task >= (int64_t)tokens * stretches) return;
   const int t = (int)(task / stretches), c0 = (int)(task % stretches) * (32 * U) + lane;
   float acc[U][V];
@@ -374,6 +385,8 @@ route_combine_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* ys, i
                           const int32_t* __restrict__ position, int tokens, int topk, int packs, int rows) {
   __shared__ float part[kRowThreads / 32][J];
   const int t = (int)blockIdx.x * (int)blockDim.y + (int)threadIdx.y;
+  dependency_wait();
+  dependents_go();
   const int lane = threadIdx.x & 31;
   const int warps = (int)blockDim.x >> 5, row_warp0 = (int)threadIdx.y * warps, my_warp = row_warp0 + ((int)threadIdx.x >> 5);
   for (int j0 = 0; j0 < topk; j0 += J) {
@@ -462,20 +475,7 @@ alphasparseStatus_t run_sort(alphasparseHandle_t h, alphasparseRoutingDescr_t r,
     if (smem > 48 * 1024) ASP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     int ctas = 1;  // a CTA per 2,048 slots (four steps of its warps), as far as a cluster goes
     while (ctas < kSortCluster && ctas * 2048 < slots) ctas *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kSortThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = h->stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ctas;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = ctas > 1 ? 1 : 0;
-    ASP_CUDA(cudaLaunchKernelEx(&cfg, kernel, ids, slots, experts, r->expert_offsets, r->position));
-    ++impl(h)->launches;
-    return ALPHA_SPARSE_STATUS_SUCCESS;
+    return launch_chained(h, kernel, dim3(ctas), dim3(kSortThreads), smem, ctas, ids, slots, experts, r->expert_offsets, r->position);
   }
   const int blocks = (int)sort_blocks(h, slots);
   int* before = reinterpret_cast<int*>((reinterpret_cast<uintptr_t>(buffer) + 15) & ~(uintptr_t)15);
@@ -485,12 +485,9 @@ alphasparseStatus_t run_sort(alphasparseHandle_t h, alphasparseRoutingDescr_t r,
     ASP_CUDA(cudaFuncSetAttribute(count, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     ASP_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   }
-  count<<<blocks, kSortThreads, smem, h->stream>>>(ids, slots, experts, before);
-  ASP_CUDA(cudaGetLastError());
-  place<<<blocks, kSortThreads, smem, h->stream>>>(ids, slots, experts, before, r->expert_offsets, r->position);
-  ASP_CUDA(cudaGetLastError());
-  impl(h)->launches += 2;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
+  const alphasparseStatus_t s = launch_chained(h, count, dim3(blocks), dim3(kSortThreads), smem, 1, ids, slots, experts, before);
+  if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  return launch_chained(h, place, dim3(blocks), dim3(kSortThreads), smem, 1, ids, slots, experts, before, r->expert_offsets, r->position);
 }
 template <typename Id>
 alphasparseStatus_t run_sort(alphasparseHandle_t h, alphasparseRoutingDescr_t r, void* buffer) {
@@ -508,12 +505,9 @@ alphasparseStatus_t run_dispatch(alphasparseHandle_t h, alphasparseRoutingDescr_
   const int64_t packs = x->cols / V, stretches = (packs + 32 * U - 1) / (32 * U);
   const int64_t blocks = row_blocks(r->tokens, stretches);
   if (blocks >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
-  route_dispatch_kernel<T, V, U><<<(unsigned)blocks, kRowThreads, 0, h->stream>>>(
+  return launch_chained(h, route_dispatch_kernel<T, V, U>, dim3((unsigned)blocks), dim3(kRowThreads), 0, 1,
       (const T*)x->values, x->ld, (T*)xs->values, xs->ld, r->position, (int)r->tokens, (int)r->topk, (int)packs,
       (int)stretches, (int)xs->rows);
-  ASP_CUDA(cudaGetLastError());
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
 template <typename T, int V>
@@ -523,12 +517,9 @@ alphasparseStatus_t run_combine(alphasparseHandle_t h, alphasparseRoutingDescr_t
   const int64_t packs = y->cols / V, stretches = (packs + 32 * U - 1) / (32 * U);
   const int64_t blocks = row_blocks(r->tokens, stretches);
   if (blocks >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
-  route_combine_kernel<T, V, U, 4><<<(unsigned)blocks, kRowThreads, 0, h->stream>>>(
+  return launch_chained(h, route_combine_kernel<T, V, U, 4>, dim3((unsigned)blocks), dim3(kRowThreads), 0, 1,
       (const T*)ys->values, ys->ld, weights, res ? (const T*)res->values : nullptr, res ? res->ld : 0, (T*)y->values,
       y->ld, r->position, (int)r->tokens, (int)r->topk, (int)packs, (int)stretches, (int)ys->rows);
-  ASP_CUDA(cudaGetLastError());
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
 template <typename T, int V>
@@ -540,13 +531,10 @@ alphasparseStatus_t run_combine_grad(alphasparseHandle_t h, alphasparseRoutingDe
   while (x < kGradThreads && x < packs) x *= 2;
   const int y = kRowThreads / x;
   const int64_t blocks = (r->tokens + y - 1) / y;
-  route_combine_grad_kernel<T, V, 4><<<(unsigned)blocks, dim3(x, y), 0, h->stream>>>(
+  return launch_chained(h, route_combine_grad_kernel<T, V, 4>, dim3((unsigned)blocks), dim3(x, y), 0, 1,
       (const T*)dy->values, dy->ld, ys ? (const T*)ys->values : nullptr, ys ? ys->ld : 0, weights,
       dys ? (T*)dys->values : nullptr, dys ? dys->ld : 0, dweights, r->position, (int)r->tokens, (int)r->topk, (int)packs,
       (int)rows);
-  ASP_CUDA(cudaGetLastError());
-  ++impl(h)->launches;
-  return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
 }  // namespace
