@@ -43,6 +43,9 @@ struct HandleImpl {
   double bf16_flops = 1.4e15, hbm_bytes = 6.5e12;
   // device flag a kernel of the expert products raises when a bounded wait expires
   int* dev_err = nullptr;
+  // polls of their waits, 0 for the default (bit 31: testing only - a copy is announced but not issued, so the waits do
+  // run out); read from ASP_WAIT_POLLS / ASP_TEST_DROP_COPY when the handle is made
+  uint32_t expert_wait = 0;
 };
 
 // Makes the handle's device current for a scope and puts the caller's back.

@@ -168,7 +168,11 @@ constexpr int kMmThreads = 384;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;    // two warps per quarter of the lanes, each half of the columns
 constexpr int kTmemCols = 512;                 // two accumulators of 256 columns
 // Polls of a bounded wait: seconds, and more than a tile of `chunks` stages can take.
-inline uint32_t wait_limit(int64_t chunks) { return (1u << 22) + (uint32_t)(chunks < (1 << 23) ? 128 * chunks : (1 << 30)); }
+inline uint32_t wait_limit(alphasparseHandle_t h, int64_t chunks) {
+  const HandleImpl* i = impl(h);
+  if (i->expert_wait) return i->expert_wait;
+  return (1u << 22) + (uint32_t)(chunks < (1 << 23) ? 128 * chunks : (1 << 30));
+}
 
 // Which contraction the kernel runs.
 enum MmKind {
@@ -195,7 +199,7 @@ struct MmArgs {
   int64_t ldb;
   int bias_type;
   int act;
-  uint32_t limit;
+  uint32_t limit;     // polls of a wait; bit 31 (kWaitDropCopy): testing
   int* err;
 };
 
@@ -376,6 +380,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   __shared__ int s_warp[kMmThreads / 32];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t limit = a.limit & ~kWaitDropCopy;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const int mblocks = (a.m_total + kTileM * CG - 1) / (kTileM * CG);
   const int jblocks = KIND == kGradW ? (a.j_total + kTileJ - 1) / kTileJ : 0;
@@ -430,7 +435,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const int box = KIND == kGradW ? 64 : a.box_rows, boxes = (half + box - 1) / box;
       const uint32_t bytes = kABytes + (uint32_t)(boxes * box * 128);
       for (int c = 0; c < x.klen; c += kKC) {
-        if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, limit))) {
           ok = false;
           break;
         }
@@ -440,7 +445,9 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           const bool own = KIND == kGradW && x.klen - c < kKC && ((x.klen - c) & 15) != 0;
           const uint32_t bar = own ? (CG == 2 ? peer_u32(tail + 8 * st, rank) : tail + 8 * st) : CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st;
           mbar_arrive_tx(bar, bytes);
-          if constexpr (KIND == kFwdT) {
+          if (a.limit & kWaitDropCopy) {
+            // testing: announced but not issued, so that every role's wait runs out
+          } else if constexpr (KIND == kFwdT) {
             tma_3d<CG>(sa, &map_a, c, m, x.e, bar);
           } else if constexpr (KIND == kFwdN) {
             tma_3d<CG>(sa, &map_a, m, c, x.e, bar);
@@ -463,7 +470,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     }
     // no stage is left with an arrival on its way to this CTA
     for (int i = 0; i < kStages && ok; ++i) {
-      ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit));
+      ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, limit));
       if (++st == kStages) {
         st = 0;
         ph ^= 1u;
@@ -480,14 +487,14 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       for (int t = first; t < total && ok; t += stride, ++n) {
         const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
         const int buf = n & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * buf, (uint32_t)(((n >> 1) & 1) ^ 1), a.limit))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * buf, (uint32_t)(((n >> 1) & 1) ^ 1), limit))) {
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + (uint32_t)buf * kTileJ, idesc = idesc0 | ((uint32_t)(x.width >> 3) << 17);
         for (int c = 0; c < x.klen; c += kKC) {
-          if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, a.limit))) {
+          if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, limit))) {
             ok = false;
             break;
           }
@@ -521,7 +528,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         chunk += chunks;
         if (chunks == 0 || (left & 15) == 0) continue;
         const int st = (chunk - 1) % kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(tail + 8 * st, (phases >> st) & 1u, a.limit))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(tail + 8 * st, (phases >> st) & 1u, limit))) {
           ok = false;
           break;
         }
@@ -547,7 +554,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const int m = x.m0 + (int)rank * kTileM + quarter * 32 + lane;
       const bool in = m < a.m_total;
       const float bias = a.bias && in ? load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type) : 0.f;
-      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * buf, (uint32_t)((n >> 1) & 1), a.limit))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * buf, (uint32_t)((n >> 1) & 1), limit))) {
         ok = false;
         break;
       }
@@ -702,6 +709,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kFewStages + 1);
   int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t limit = a.limit & ~kWaitDropCopy;
   const uint32_t rank = size > 1 ? cluster_rank() : 0u;
   const int mblocks = (a.m_total + kTileM - 1) / kTileM, t = (int)blockIdx.x / size;
   if (tid == 0) {
@@ -739,14 +747,16 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     int st = 0;
     uint32_t ph = 0;
     for (int c = c0; c < c1; ++c) {
-      if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, a.limit))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, limit))) {
         ok = false;
         break;
       }
       if (elect_one()) {
         const uint32_t sa = base + st * kStage, sb = sa + kABytes, bar = full + 8 * st;
         mbar_arrive_tx(bar, bytes);
-        if constexpr (KIND == kFwdT) {
+        if (a.limit & kWaitDropCopy) {
+          // testing, as in the kernel above
+        } else if constexpr (KIND == kFwdT) {
           tma_3d<1>(sa, &map_a, c * kKC, x.m0, x.e, bar);
         } else {
           tma_3d<1>(sa, &map_a, x.m0, c * kKC, x.e, bar);
@@ -767,7 +777,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const uint32_t idesc = (1u << 4) | a.types | kMajor | ((uint32_t)(x.width >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
     constexpr uint32_t kStepA = KIND == kFwdT ? 2u : 128u;
     for (int c = c0; c < c1; ++c) {
-      if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, a.limit))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, limit))) {
         ok = false;
         break;
       }
@@ -793,7 +803,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   float bias = 0.f;
   if (epilogue) {
     if (a.bias && in) bias = load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type);
-    ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0u, a.limit));
+    ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0u, limit));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (ok) {
       // every MMA of this CTA is done: the ring's memory takes the sums, [row][column]
@@ -1093,7 +1103,7 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   if (z) a.z = z->values, a.ldz = z->ld;
   if (bias) a.bias = bias->values, a.ldb = bias->ld, a.bias_type = (int)bias->data_type;
   a.act = (int)act;
-  a.limit = wait_limit(shape.k / kKC);
+  a.limit = wait_limit(h, shape.k / kKC);
   a.err = impl(h)->dev_err;
   CUtensorMap mw = {}, mx = {};
   if (shape.k > 0) {
@@ -1144,7 +1154,7 @@ alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparse
   a.types = type_bits(x->data_type);
   a.y = dw->values;
   a.ldy = dw->ld;
-  a.limit = wait_limit(x->rows / kKC);
+  a.limit = wait_limit(h, x->rows / kKC);
   a.err = impl(h)->dev_err;
   CUtensorMap mm = {}, mj = {};
   if (x->rows > 0) {

@@ -86,6 +86,9 @@ alphasparseStatus_t alphasparseGetHandle(alphasparseHandle_t* handle) {
   if (!impl(h)->dev_err) {
     ASP_CUDA(cudaMalloc((void**)&impl(h)->dev_err, sizeof(int)));
     ASP_CUDA(cudaMemsetAsync(impl(h)->dev_err, 0, sizeof(int), h->stream));
+    const int polls = env_int("ASP_WAIT_POLLS", 0);
+    impl(h)->expert_wait = polls > 0 ? (uint32_t)polls & kWaitPollMask : 0;
+    if (env_int("ASP_TEST_DROP_COPY", 0)) impl(h)->expert_wait = (impl(h)->expert_wait ? impl(h)->expert_wait : 1u << 12) | kWaitDropCopy;
   }
   asp_init_kernel<<<1, 1, 0, h->stream>>>();
   ASP_CUDA(cudaGetLastError());

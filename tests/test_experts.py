@@ -389,10 +389,12 @@ def test_dispatch_passes_over_bad_positions(h):
 # ---- the products -------------------------------------------------------------------------------
 
 # counts per segment, K, N: one row; one token's choice of experts; ragged with empty segments at both ends; a plain dense
-# layer; tiles cut in every direction; K from nothing up; many segments
+# layer; tiles cut in every direction; K from nothing up; many segments, as many as there may be; nothing but empty ones; more tiles
+# than the device holds at once; both kernels for few rows, with and without a shared contraction
 PRODUCTS = [([1], 64, 64), ([0, 1, 0, 1, 1], 256, 200), ([0, 130, 1, 0, 257, 64, 0], 192, 136), ([300], 512, 384), ([17], 1024, 640),
             ([5, 9], 8, 8), ([3, 0, 2], 1, 1), ([70, 3], 0, 24), ([33, 40], 1000, 515), ([129, 255, 256], 72, 264),
-            ([2] * 200 + [0] * 100 + [3] * 57, 40, 24), ([600, 1], 2048, 128)]
+            ([2] * 200 + [0] * 100 + [3] * 57, 40, 24), ([600, 1], 2048, 128), ([0, 0, 0], 64, 40), ([20] * 1023 + [40], 24, 16),
+            ([10] * 33, 136, 72), ([700, 900, 257, 0, 1200], 320, 2000), ([64, 50, 1], 1096, 3000), ([48] * 40, 128, 1032)]
 
 
 def product_inputs(counts, k, n, op, dt, seed, pad, shift, tail):
@@ -541,6 +543,40 @@ def test_offsets_outside_the_rows(h):
     api.expert_act_grad(h, api.DnMat(y), None, None, off, api.ACT_NONE, api.DnMat(db),
                         buffer(api.expert_act_grad_buffer_size(h, api.DnMat(y), off, api.ACT_NONE, api.DnMat(db))))
     assert db[1].eq(0).all()
+
+
+@pytest.mark.gpu
+def test_waits_that_run_out_are_reported(monkeypatch):
+    """Failure detection without a fault: the producers announce their copies and do not issue them, so every role's bounded
+    wait runs out, the blocks raise the handle's flag, free their tensor memory and leave.  A fresh handle computes."""
+    x = torch.randn(600, 256, device="cuda").to(torch.bfloat16)
+    w = torch.randn(512, 256, device="cuda").to(torch.bfloat16)
+    y = torch.zeros(600, 512, dtype=torch.bfloat16, device="cuda")
+    dw = torch.zeros(512, 256, dtype=torch.bfloat16, device="cuda")
+
+    def calls(h):
+        api.expert_mm(h, api.DnMat(x), api.DnMat(w), api.DnMat(y))                         # the pair kernel
+        api.expert_mm(h, api.DnMat(x[:5]), api.DnMat(w), api.DnMat(y[:5]))                 # few rows
+        api.expert_mm_grad_weight(h, api.DnMat(x[:500]), api.DnMat(y[:500]), api.DnMat(dw))  # with a tail to clear
+
+    monkeypatch.setenv("ASP_TEST_DROP_COPY", "1")
+    monkeypatch.setenv("ASP_WAIT_POLLS", "64")
+    flags = []
+    for i in range(3):
+        broken = api.Handle()
+        (lambda: api.expert_mm(broken, api.DnMat(x), api.DnMat(w), api.DnMat(y)),
+         lambda: api.expert_mm(broken, api.DnMat(x[:5]), api.DnMat(w), api.DnMat(y[:5])),
+         lambda: api.expert_mm_grad_weight(broken, api.DnMat(x[:500]), api.DnMat(y[:500]), api.DnMat(dw)))[i]()
+        flags.append(api.device_error(broken))
+    monkeypatch.delenv("ASP_TEST_DROP_COPY")
+    monkeypatch.delenv("ASP_WAIT_POLLS")
+    assert flags == [1, 1, 1]
+    fresh = api.Handle()
+    calls(fresh)
+    want = x.double() @ w.double().t()
+    mag = x.double().abs() @ w.double().abs().t()
+    close(y, want, u(torch.bfloat16) * want.abs() + 256 * 2 * U * mag)
+    assert api.device_error(fresh) == 0
 
 
 # ---- the epilogue's gradient ---------------------------------------------------------------------
