@@ -3,10 +3,19 @@
 //   Z[p,n] = sum_k X[p,k] op(W_e)[k,n] + bias[e,n],   Y[p,n] = act(Z[p,n]) + R[p,n]   for p in segment e
 //   dW_e   = dZ_e^T X_e  (or its transpose)
 //
-// One persistent kernel for both.  The MMA's M side (lanes of tensor memory) is always the output's
+// expert_mm_kernel runs both: persistent pairs of CTAs whose tcgen05.mma (M = 256, N up to 256) shares the N operand between the two
+// SMs, operands staged by TMA in a ring of six 32 KB stages per CTA, two accumulators in tensor memory so that a tile's epilogue runs
+// behind the next tile's MMAs.  expert_mm_few_kernel takes products of few rows, whose work is the weights' bytes.
+// The MMA's M side (lanes of tensor memory) is always the output's
 // contiguous dimension, its N side the output's rows: a warp of the epilogue then writes 32
 // neighbouring elements of a row, and the N of an MMA, which the instruction takes in steps of 16,
 // follows a ragged segment closely.
+//
+// What bounds the pair kernel: power.  In a run of seconds (1,000 W, about 1.35 GHz) 32,768 x 2,048 times 2,048 x 4,096 in bf16 takes
+// 441-446 us (1,235 TFLOP/s) against 417 us for a library product of the same sizes; in short bursts 1,370 TFLOP/s, 1,450 at
+// K = N = 4,096.  Spread over 32 experts it takes 487 us (520 MB more of weights from HBM), with uneven segments 518 us.  The tile
+// order matters for that reason: pairs that work at a time take all column blocks of few row tiles (448 us); groups of eight
+// column blocks 452, of four 479 us (more distinct rows of X cross the fabric).
 #include <cuda.h>
 
 #include <atomic>
@@ -46,16 +55,17 @@ __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Bounded wait on a barrier of this CTA: false if the phase did not complete within `limit` polls.
+// Bounded wait on a barrier of this CTA: false if the phase did not complete within `limit` polls.  A poll parks the warp for up to two
+// microseconds or until the phase completes: a warp that polls flat out costs power, and power is what limits the products.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
   for (uint32_t i = 0; i < limit; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "r"(bar), "r"(parity), "r"(2000)
         : "memory");
     if (ok) return true;
   }
@@ -75,6 +85,7 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 // TMA loads into this CTA's shared memory.  The .cta_group::2 form may complete on a barrier of either CTA of the pair.
+// CG: CTAs of the MMA.
 template <int CG>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   if constexpr (CG == 2)
@@ -161,8 +172,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 constexpr int kKC = 64;                        // contraction per stage: 128 bytes of a 16-bit type
 constexpr int kTileM = 128;                    // M of a CTA: lanes of tensor memory
 constexpr int kTileJ = 256;                    // N of an MMA, at most: rows of the output per tile
-constexpr int kMmStages = 6;
+constexpr int kPairM = 2 * kTileM;             // columns of the output per tile
 constexpr int kABytes = kTileM * kKC * 2;      // 16 KB
+constexpr int kMmStages = 6;
+constexpr int kMmStage = kABytes + kTileJ / 2 * kKC * 2;  // a CTA's 128 columns of M and its half of N: 32 KB
 constexpr int kBoxBytes = 64 * 128;            // an MN-major box
 constexpr int kMmThreads = 384;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;    // two warps per quarter of the lanes, each half of the columns
@@ -171,7 +184,7 @@ constexpr int kTmemCols = 512;                 // two accumulators of 256 column
 inline uint32_t wait_limit(alphasparseHandle_t h, int64_t chunks) {
   const HandleImpl* i = impl(h);
   if (i->expert_wait) return i->expert_wait;
-  return (1u << 22) + (uint32_t)(chunks < (1 << 23) ? 128 * chunks : (1 << 30));
+  return (1u << 21) + (uint32_t)(chunks < (1 << 23) ? 128 * chunks : (1 << 30));
 }
 
 // Which contraction the kernel runs.
@@ -276,21 +289,21 @@ __device__ __forceinline__ void row_tile(int j, int segments, const int* s_off, 
 }
 
 // Tile t of the launch.  Whole warp; every lane gets the same answer.
-template <int KIND, int CG>
+template <int KIND>
 __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off, const int* s_tile, int mblocks, int jblocks) {
   Tile x;
   if constexpr (KIND == kGradW) {
     const int per = mblocks * jblocks;
     x.e = t / per;
     const int i = t % per, j = i / mblocks;
-    x.m0 = (i % mblocks) * (kTileM * CG);
+    x.m0 = (i % mblocks) * kPairM;
     const int left = a.j_total - j * kTileJ;
     x.rows = left < kTileJ ? left : kTileJ;
     x.row0 = j * kTileJ;  // within the block of dW
     x.k0 = s_off[x.e];
     x.klen = s_off[x.e + 1] > x.k0 ? s_off[x.e + 1] - x.k0 : 0;
   } else {
-    x.m0 = (t % mblocks) * (kTileM * CG);
+    x.m0 = (t % mblocks) * kPairM;
     row_tile(t / mblocks, a.segments, s_off, s_tile, x);
     x.k0 = 0;
     x.klen = a.k;
@@ -359,21 +372,18 @@ __device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int 
 }
 
 // Warp roles: 0 TMA producer, 1 MMA issuer, 2 clearing of ragged tails (kGradW), 4-11 epilogue.
-template <int KIND, int CG, typename TO>
+template <int KIND, typename TO>
 __global__ void __launch_bounds__(kMmThreads, 1)
 expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ MmArgs a) {
-  constexpr int kBBytes = kTileJ / CG * kKC * 2;
-  constexpr int kStage = kABytes + kBBytes;
   extern __shared__ unsigned char smem_raw[];
   // swizzled tiles need a 1,024-byte aligned base; the offset is the same in both CTAs of a pair
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gen = smem_raw + (base - raw);
-  constexpr int kStages = CG == 2 ? kMmStages : 4;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(gen + kStages * kStage);
-  const uint32_t bar0 = base + kStages * kStage;
-  const uint32_t full = bar0, empty = bar0 + 8 * kStages, tail = bar0 + 16 * kStages, acc_full = bar0 + 24 * kStages,
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gen + kMmStages * kMmStage);
+  const uint32_t bar0 = base + kMmStages * kMmStage;
+  const uint32_t full = bar0, empty = bar0 + 8 * kMmStages, tail = bar0 + 16 * kMmStages, acc_full = bar0 + 24 * kMmStages,
                  acc_empty = acc_full + 16;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 3 * kStages + 4);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 3 * kMmStages + 4);
   int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
   int* s_off = s_fail + 1;                             // segments + 1
   int* s_tile = s_off + ALPHASPARSE_MAX_EXPERTS + 1;   // segments + 1
@@ -381,24 +391,24 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t limit = a.limit & ~kWaitDropCopy;
-  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
-  const int mblocks = (a.m_total + kTileM * CG - 1) / (kTileM * CG);
+  const uint32_t rank = cluster_rank();
+  const int mblocks = (a.m_total + kPairM - 1) / kPairM;
   const int jblocks = KIND == kGradW ? (a.j_total + kTileJ - 1) / kTileJ : 0;
 
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + 8 * i, CG);   // an arrival per CTA
+    for (int i = 0; i < kMmStages; ++i) {
+      mbar_init(full + 8 * i, 2);  // an arrival per CTA
       mbar_init(empty + 8 * i, 1);
       mbar_init(tail + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8 * i, 1);
-      mbar_init(acc_empty + 8 * i, CG * kEpiWarps);
+      mbar_init(acc_empty + 8 * i, 2 * kEpiWarps);
     }
     *s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc<CG>(smem_u32(s_tmem), kTmemCols);
+  if (warp == 1) tmem_alloc<2>(smem_u32(s_tmem), kTmemCols);
   if (tid == 32 * 3) {
     prefetch_map(&map_a);
     prefetch_map(&map_b);
@@ -417,10 +427,10 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // the peer's barriers are ready
+  cluster_sync();  // the peer's barriers are ready
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *s_tmem;
-  const int first = (int)blockIdx.x / CG, stride = (int)gridDim.x / CG;
+  const int first = (int)blockIdx.x / 2, stride = (int)gridDim.x / 2;
   bool ok = true;
 
   if (warp == 0) {
@@ -428,9 +438,9 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     int st = 0;
     uint32_t ph = 0;
     for (int t = first; t < total && ok; t += stride) {
-      const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+      const Tile x = tile_of<KIND>(t, a, s_off, s_tile, mblocks, jblocks);
       const int m = x.m0 + (int)rank * kTileM;
-      const int half = x.width / CG;  // rows of the B operand in this CTA
+      const int half = x.width / 2;  // rows of the B operand in this CTA
       const int j = x.row0 + (int)rank * half;
       const int box = KIND == kGradW ? 64 : a.box_rows, boxes = (half + box - 1) / box;
       const uint32_t bytes = kABytes + (uint32_t)(boxes * box * 128);
@@ -440,38 +450,38 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           break;
         }
         if (elect_one()) {
-          const uint32_t sa = base + st * kStage, sb = sa + kABytes;
+          const uint32_t sa = base + st * kMmStage, sb = sa + kABytes;
           // a last chunk that has to be cleared completes on the CTA's own barrier; warp 2 passes it on
           const bool own = KIND == kGradW && x.klen - c < kKC && ((x.klen - c) & 15) != 0;
-          const uint32_t bar = own ? (CG == 2 ? peer_u32(tail + 8 * st, rank) : tail + 8 * st) : CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st;
+          const uint32_t bar = peer_u32(own ? tail + 8 * st : full + 8 * st, own ? rank : 0);
           mbar_arrive_tx(bar, bytes);
           if (a.limit & kWaitDropCopy) {
             // testing: announced but not issued, so that every role's wait runs out
           } else if constexpr (KIND == kFwdT) {
-            tma_3d<CG>(sa, &map_a, c, m, x.e, bar);
+            tma_3d<2>(sa, &map_a, c, m, x.e, bar);
           } else if constexpr (KIND == kFwdN) {
-            tma_3d<CG>(sa, &map_a, m, c, x.e, bar);
-            tma_3d<CG>(sa + kBoxBytes, &map_a, m + 64, c, x.e, bar);
+            tma_3d<2>(sa, &map_a, m, c, x.e, bar);
+            tma_3d<2>(sa + kBoxBytes, &map_a, m + 64, c, x.e, bar);
           } else {
-            tma_2d<CG>(sa, &map_a, m, x.k0 + c, bar);
-            tma_2d<CG>(sa + kBoxBytes, &map_a, m + 64, x.k0 + c, bar);
+            tma_2d<2>(sa, &map_a, m, x.k0 + c, bar);
+            tma_2d<2>(sa + kBoxBytes, &map_a, m + 64, x.k0 + c, bar);
           }
           for (int b = 0; b < boxes; ++b) {
-            if constexpr (KIND == kGradW) tma_2d<CG>(sb + b * kBoxBytes, &map_b, j + b * 64, x.k0 + c, bar);
-            else tma_2d<CG>(sb + b * box * 128, &map_b, c, j + b * box, bar);
+            if constexpr (KIND == kGradW) tma_2d<2>(sb + b * kBoxBytes, &map_b, j + b * 64, x.k0 + c, bar);
+            else tma_2d<2>(sb + b * box * 128, &map_b, c, j + b * box, bar);
           }
         }
         __syncwarp();
-        if (++st == kStages) {
+        if (++st == kMmStages) {
           st = 0;
           ph ^= 1u;
         }
       }
     }
     // no stage is left with an arrival on its way to this CTA
-    for (int i = 0; i < kStages && ok; ++i) {
+    for (int i = 0; i < kMmStages && ok; ++i) {
       ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ph ^ 1u, limit));
-      if (++st == kStages) {
+      if (++st == kMmStages) {
         st = 0;
         ph ^= 1u;
       }
@@ -482,10 +492,10 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       int st = 0, n = 0;
       uint32_t ph = 0;
       constexpr uint32_t kMajor = KIND == kFwdN ? (1u << 15) : KIND == kGradW ? (1u << 15) | (1u << 16) : 0u;
-      const uint32_t idesc0 = (1u << 4) | a.types | kMajor | ((uint32_t)(kTileM * CG >> 4) << 24);
+      const uint32_t idesc0 = (1u << 4) | a.types | kMajor | ((uint32_t)(kPairM >> 4) << 24);
       constexpr uint32_t kStepA = KIND == kFwdT ? 2u : 128u, kStepB = KIND == kGradW ? 128u : 2u;  // 16 elements of k, in 16 bytes
       for (int t = first; t < total && ok; t += stride, ++n) {
-        const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+        const Tile x = tile_of<KIND>(t, a, s_off, s_tile, mblocks, jblocks);
         const int buf = n & 1;
         if (!__all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * buf, (uint32_t)(((n >> 1) & 1) ^ 1), limit))) {
           ok = false;
@@ -499,21 +509,21 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             break;
           }
           // (zeros that a warp of the peer stored in its tail)
-          if (KIND == kGradW && CG == 2 && x.klen - c < kKC) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          if (KIND == kGradW && x.klen - c < kKC) asm volatile("fence.acq_rel.cluster;" ::: "memory");
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (elect_one()) {
-            const uint64_t da = umma_desc(base + st * kStage, kBoxBytes), db = umma_desc(base + st * kStage + kABytes, kBoxBytes);
+            const uint64_t da = umma_desc(base + st * kMmStage, kBoxBytes), db = umma_desc(base + st * kMmStage + kABytes, kBoxBytes);
             const int left = x.klen - c, steps = left >= kKC ? kKC / 16 : (left + 15) / 16;
-            for (int s = 0; s < steps; ++s) umma<CG>(d, da + s * kStepA, db + s * kStepB, idesc, c > 0 || s > 0 ? 1u : 0u);
-            umma_commit<CG>(empty + 8 * st);
+            for (int s = 0; s < steps; ++s) umma<2>(d, da + s * kStepA, db + s * kStepB, idesc, c > 0 || s > 0 ? 1u : 0u);
+            umma_commit<2>(empty + 8 * st);
           }
           __syncwarp();
-          if (++st == kStages) {
+          if (++st == kMmStages) {
             st = 0;
             ph ^= 1u;
           }
         }
-        if (ok && elect_one()) umma_commit<CG>(acc_full + 8 * buf);
+        if (ok && elect_one()) umma_commit<2>(acc_full + 8 * buf);
         __syncwarp();
       }
     }
@@ -523,24 +533,24 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       int chunk = 0;
       uint32_t phases = 0;  // of the tail barriers, a bit per stage
       for (int t = first; t < total && ok; t += stride) {
-        const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+        const Tile x = tile_of<KIND>(t, a, s_off, s_tile, mblocks, jblocks);
         const int chunks = (x.klen + kKC - 1) / kKC, left = x.klen - (chunks - 1) * kKC;
         chunk += chunks;
         if (chunks == 0 || (left & 15) == 0) continue;
-        const int st = (chunk - 1) % kStages;
+        const int st = (chunk - 1) % kMmStages;
         if (!__all_sync(0xffffffffu, mbar_wait(tail + 8 * st, (phases >> st) & 1u, limit))) {
           ok = false;
           break;
         }
         phases ^= 1u << st;
         const int to = (left + 15) & ~15, n16 = (to - left) * 8;   // 16-byte words per box
-        const int boxes = 2 + (x.width / CG + 63) / 64;
-        unsigned char* s = gen + st * kStage;
+        const int boxes = 2 + (x.width / 2 + 63) / 64;
+        unsigned char* s = gen + st * kMmStage;
         for (int i = lane; i < n16 * boxes; i += 32)  // whole rows of 128 bytes: the swizzle does not matter
           *reinterpret_cast<uint4*>(s + (i / n16) * kBoxBytes + left * 128 + (i % n16) * 16) = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(CG == 2 ? peer_u32(full + 8 * st, 0) : full + 8 * st);
+        if (lane == 0) mbar_arrive(peer_u32(full + 8 * st, 0));
         __syncwarp();
       }
     }
@@ -549,7 +559,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int quarter = warp & 3, half = (warp - kEpiWarp0) >> 2;
     int n = 0;
     for (int t = first; t < total && ok; t += stride, ++n) {
-      const Tile x = tile_of<KIND, CG>(t, a, s_off, s_tile, mblocks, jblocks);
+      const Tile x = tile_of<KIND>(t, a, s_off, s_tile, mblocks, jblocks);
       const int buf = n & 1;
       const int m = x.m0 + (int)rank * kTileM + quarter * 32 + lane;
       const bool in = m < a.m_total;
@@ -568,7 +578,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         default: finish_tile<TO, ALPHASPARSE_ACT_NONE>(a, x, m, half, d, in, bias, out_row0); break;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      if (lane == 0) mbar_arrive(CG == 2 ? peer_u32(acc_empty + 8 * buf, 0) : acc_empty + 8 * buf);
+      if (lane == 0) mbar_arrive(peer_u32(acc_empty + 8 * buf, 0));
     }
   }
   __syncwarp();
@@ -580,9 +590,9 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (tid == 0) *a.err = 1;
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   }
-  if constexpr (CG == 2) cluster_sync();  // the peer's MMAs read this CTA's shared memory, its arrivals land here
+  cluster_sync();  // the peer's MMAs read this CTA's shared memory, its arrivals land here
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 1) tmem_free<CG>(tmem, kTmemCols);
+  if (warp == 1) tmem_free<2>(tmem, kTmemCols);
 }
 
 // ---- few rows: the weights' bytes are the work ----------------------------------------------------
@@ -950,25 +960,23 @@ alphasparseStatus_t allow_smem(K* kernel, int bytes, int device, std::atomic<uin
   return ALPHA_SPARSE_STATUS_SUCCESS;
 }
 
-template <int KIND, int CG, typename TO>
+template <int KIND, typename TO>
 alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles) {
-  constexpr int stages = CG == 2 ? kMmStages : 4;
-  constexpr size_t smem = 1024 + (size_t)stages * (kABytes + kTileJ / CG * kKC * 2) + 8 * (3 * stages + 4) + 8 +
-                          8 * (ALPHASPARSE_MAX_EXPERTS + 1);
+  constexpr size_t smem = 1024 + (size_t)kMmStages * kMmStage + 8 * (3 * kMmStages + 4) + 8 + 8 * (ALPHASPARSE_MAX_EXPERTS + 1);
   static std::atomic<uint64_t> done{0};
-  const auto kernel = expert_mm_kernel<KIND, CG, TO>;
+  const auto kernel = expert_mm_kernel<KIND, TO>;
   const alphasparseStatus_t s = allow_smem(kernel, (int)smem, h->device, &done);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
-  const int64_t most = impl(h)->sm_count / CG;
-  return launch_chained(h, kernel, dim3((unsigned)((tiles < most ? tiles : most) * CG)), dim3(kMmThreads), smem, CG, ma, mb, a);
+  const int64_t most = impl(h)->sm_count / 2;
+  return launch_chained(h, kernel, dim3((unsigned)((tiles < most ? tiles : most) * 2)), dim3(kMmThreads), smem, 2, ma, mb, a);
 }
-template <int KIND, int CG>
+template <int KIND>
 alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
                               alphasparseDataType out) {
   switch (out) {
-    case ALPHA_R_32F: return launch_mm<KIND, CG, float>(h, ma, mb, a, tiles);
-    case ALPHA_R_16F: return launch_mm<KIND, CG, __half>(h, ma, mb, a, tiles);
-    default: return launch_mm<KIND, CG, __nv_bfloat16>(h, ma, mb, a, tiles);
+    case ALPHA_R_32F: return launch_mm<KIND, float>(h, ma, mb, a, tiles);
+    case ALPHA_R_16F: return launch_mm<KIND, __half>(h, ma, mb, a, tiles);
+    default: return launch_mm<KIND, __nv_bfloat16>(h, ma, mb, a, tiles);
   }
 }
 
@@ -1005,7 +1013,7 @@ struct MmShape {
 // SMs' pairs or less leave the HBM idle (one 4,096 x 4,096 layer, 32 / 128 / 256 rows: 15 / 18 / 24 us against 26 / 28 / 29; 512 rows
 // 35 against 30; eight 2,048 x 2,048 layers, 256 rows: 23 against 22).
 int few_rows(alphasparseHandle_t h, const MmShape& s, int64_t filled) {
-  const int64_t pairs = (s.rows / kTileJ + filled) * ((s.n + 2 * kTileM - 1) / (2 * kTileM));
+  const int64_t pairs = (s.rows / kTileJ + filled) * ((s.n + kPairM - 1) / kPairM);
   if (s.rows <= 16 * filled) return 1;
   return s.rows <= 256 * filled && pairs * 3 <= impl(h)->sm_count ? 2 : 0;
 }
@@ -1117,8 +1125,8 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
       return nk ? launch_few<kFwdT, 16>(h, mw, mx, a, tiles, y->data_type) : launch_few<kFwdN, 16>(h, mw, mx, a, tiles, y->data_type);
     return nk ? launch_few<kFwdT, 64>(h, mw, mx, a, tiles, y->data_type) : launch_few<kFwdN, 64>(h, mw, mx, a, tiles, y->data_type);
   }
-  const int64_t tiles = (shape.rows / kTileJ + filled) * ((shape.n + 2 * kTileM - 1) / (2 * kTileM));
-  return nk ? launch_mm<kFwdT, 2>(h, mw, mx, a, tiles, y->data_type) : launch_mm<kFwdN, 2>(h, mw, mx, a, tiles, y->data_type);
+  const int64_t tiles = (shape.rows / kTileJ + filled) * ((shape.n + kPairM - 1) / kPairM);
+  return nk ? launch_mm<kFwdT>(h, mw, mx, a, tiles, y->data_type) : launch_mm<kFwdN>(h, mw, mx, a, tiles, y->data_type);
 }
 
 alphasparseStatus_t alphasparseExpertMM_gradW_bufferSize(alphasparseHandle_t h, alphasparseOperation_t op,
@@ -1161,9 +1169,9 @@ alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparse
     if ((s = tensor_map(&mm, om, 0, 64, kKC)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
     if ((s = tensor_map(&mj, oj, 0, 64, kKC)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   }
-  const int64_t tiles = segments * ((m->cols + 2 * kTileM - 1) / (2 * kTileM)) * ((j->cols + kTileJ - 1) / kTileJ);
+  const int64_t tiles = segments * ((m->cols + kPairM - 1) / kPairM) * ((j->cols + kTileJ - 1) / kTileJ);
   if (tiles >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
-  return launch_mm<kGradW, 2>(h, mm, mj, a, tiles, dw->data_type);
+  return launch_mm<kGradW>(h, mm, mj, a, tiles, dw->data_type);
 }
 
 }  // extern "C"

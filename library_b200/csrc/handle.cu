@@ -52,12 +52,16 @@ alphasparseStatus_t alphasparseGetHandle(alphasparseHandle_t* handle) {
   }
   alphasparseHandle_t h = *handle;
   ASP_CUDA(cudaSetDevice(h->device));
-  cudaDeviceProp prop;
-  ASP_CUDA(cudaGetDeviceProperties(&prop, h->device));
-  if (prop.major < 10) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;  // sm_100a code only
-  h->wavefront_size = prop.warpSize;
-  impl(h)->sm_count = prop.multiProcessorCount;
-  impl(h)->smem_optin = prop.sharedMemPerBlockOptin;
+  // (single attributes: the whole property structure takes milliseconds to fill)
+  int major = 0, warp = 0, sms = 0, smem_optin = 0;
+  ASP_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, h->device));
+  ASP_CUDA(cudaDeviceGetAttribute(&warp, cudaDevAttrWarpSize, h->device));
+  ASP_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, h->device));
+  ASP_CUDA(cudaDeviceGetAttribute(&smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, h->device));
+  if (major < 10) return ALPHA_SPARSE_STATUS_NOT_SUPPORTED;  // sm_100a code only
+  h->wavefront_size = warp;
+  impl(h)->sm_count = sms;
+  impl(h)->smem_optin = (size_t)smem_optin;
   {
     // dense bf16: 8192 flop per clock per SM on this architecture, of which a long-running kernel
     // sustains about 0.62 under the power cap; HBM: double data rate over the bus, of which a
@@ -67,7 +71,7 @@ alphasparseStatus_t alphasparseGetHandle(alphasparseHandle_t* handle) {
         cudaDeviceGetAttribute(&mem_khz, cudaDevAttrMemoryClockRate, h->device) == cudaSuccess &&
         cudaDeviceGetAttribute(&bus_bits, cudaDevAttrGlobalMemoryBusWidth, h->device) == cudaSuccess &&
         sm_khz > 0 && mem_khz > 0 && bus_bits > 0) {
-      impl(h)->bf16_flops = 0.62 * 8192.0 * prop.multiProcessorCount * (double)sm_khz * 1e3;
+      impl(h)->bf16_flops = 0.62 * 8192.0 * sms * (double)sm_khz * 1e3;
       impl(h)->hbm_bytes = 0.8 * 2.0 * (double)mem_khz * 1e3 * (bus_bits / 8.0);
     }
   }
