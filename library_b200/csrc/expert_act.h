@@ -60,6 +60,55 @@ __device__ __forceinline__ float activate(float z) {
   return z;
 }
 
+// Two values at once, for kernels whose arithmetic counts: packed pairs take one instruction for two fused multiply-adds (the same
+// rounding as the scalar form), and the two reciprocals share one: 1/a = b/(ab).  The denominators lie in [1, 6.2] whatever z is
+// (fminf drops a NaN), so neither value can disturb the other.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+
+template <int ACT>
+__device__ __forceinline__ void activate2(float& z0, float& z1) {
+  if constexpr (ACT == ALPHASPARSE_ACT_GELU) {
+    const float a0 = fminf(fabsf(z0), 20.f), a1 = fminf(fabsf(z1), 20.f);
+    const uint64_t az = pack2(a0, a1);
+    float d0, d1;
+    unpack2(fma2(az, both(0.26f), both(1.f)), d0, d1);
+    const uint64_t t = mul2(both(rcp_fast(d0 * d1)), pack2(d1, d0));
+    uint64_t q = both(0.0302303012f);
+    q = fma2(q, t, both(-0.151494438f));
+    q = fma2(q, t, both(0.248733209f));
+    q = fma2(q, t, both(-0.147789338f));
+    q = fma2(q, t, both(0.158758764f));
+    q = fma2(q, t, both(0.0519648210f));
+    q = fma2(q, t, both(0.102788682f));
+    q = fma2(q, t, both(0.103050974f));
+    q = fma2(q, t, both(0.103757022f));
+    float x0, x1, p0, p1;
+    unpack2(mul2(mul2(az, az), both(-0.5f * kLog2e)), x0, x1);
+    unpack2(mul2(mul2(q, t), pack2(exp2_fast(x0), exp2_fast(x1))), p0, p1);
+    z0 = z0 < -20.f ? 0.f : z0 * (z0 < 0.f ? p0 : 1.f - p0);
+    z1 = z1 < -20.f ? 0.f : z1 * (z1 < 0.f ? p1 : 1.f - p1);
+  } else {
+    z0 = activate<ACT>(z0);
+    z1 = activate<ACT>(z1);
+  }
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == ALPHASPARSE_ACT_RELU) return z > 0.f ? 1.f : 0.f;

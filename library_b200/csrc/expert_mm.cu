@@ -177,8 +177,9 @@ constexpr int kABytes = kTileM * kKC * 2;      // 16 KB
 constexpr int kMmStages = 6;
 constexpr int kMmStage = kABytes + kTileJ / 2 * kKC * 2;  // a CTA's 128 columns of M and its half of N: 32 KB
 constexpr int kBoxBytes = 64 * 128;            // an MN-major box
-constexpr int kMmThreads = 384;
-constexpr int kEpiWarp0 = 4, kEpiWarps = 8;    // two warps per quarter of the lanes, each half of the columns
+constexpr int kEpiParts = 2;                   // epilogue warps per quarter of the lanes
+constexpr int kEpiWarp0 = 4, kEpiWarps = 4 * kEpiParts;
+constexpr int kMmThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;                 // two accumulators of 256 columns
 // Polls of a bounded wait: seconds, and more than a tile of `chunks` stages can take.
 inline uint32_t wait_limit(alphasparseHandle_t h, int64_t chunks) {
@@ -315,12 +316,12 @@ __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off
 constexpr int kCols = 16;  // (32 at a time spilled registers)
 // The epilogue of kCols rows (n of them exist, all if FULL) of output column m, from row `row` of the output on: v holds the
 // sums.  Each optional operand is one guarded loop, not a test per element.
-template <typename TO, bool FULL>
+template <typename TO>
 __device__ __forceinline__ void load_residual(const MmArgs& a, int64_t row, int m, int n, TO (&res)[kCols]) {
   const TO* r = (const TO*)a.r + row * a.ldr + m;
 #pragma unroll
   for (int c = 0; c < kCols; ++c, r += a.ldr)
-    if (FULL || c < n) res[c] = *r;
+    if (c < n) res[c] = *r;
 }
 template <typename TO, int ACT, bool FULL>
 __device__ __forceinline__ void finish_values(const MmArgs& a, int64_t row, int m, int n, float bias, const TO (&res)[kCols],
@@ -334,7 +335,7 @@ __device__ __forceinline__ void finish_values(const MmArgs& a, int64_t row, int 
       if (FULL || c < n) *z = Wide<TO>::down(v[c]);
   }
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) v[c] = activate<ACT>(v[c]);
+  for (int c = 0; c < kCols; c += 2) activate2<ACT>(v[c], v[c + 1]);
   if (a.r) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
@@ -345,33 +346,34 @@ __device__ __forceinline__ void finish_values(const MmArgs& a, int64_t row, int 
   for (int c = 0; c < kCols; ++c, y += a.ldy)
     if (FULL || c < n) *y = Wide<TO>::down(v[c]);
 }
-template <typename TO, int ACT, bool FULL>
-__device__ __forceinline__ void finish_columns(const MmArgs& a, const Tile& x, int m, int c0, uint32_t tmem, bool in, float bias,
-                                               int64_t out_row0) {
-  const int n = FULL ? kCols : x.rows - c0;
-  const int64_t row = out_row0 + c0;
-  TO res[kCols];
-  if (a.r && in) load_residual<TO, FULL>(a, row, m, n, res);  // asked for before the accumulators are waited on
-  uint32_t acc[kCols];
-  tmem_ld16(tmem + (uint32_t)c0, acc);
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  if (!in) return;
-  float v[kCols];
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) v[c] = x.klen == 0 ? 0.f : __uint_as_float(acc[c]);  // an empty sum: no MMA wrote them
-  finish_values<TO, ACT, FULL>(a, row, m, n, bias, res, v);
-}
+// A warp's share of a tile: every kEpiParts-th block of kCols rows.  res holds the residual of the first; that of the next block is
+// asked for before a block is finished, so that its latency passes behind the block's arithmetic.
 template <typename TO, int ACT>
-__device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int m, int half, uint32_t tmem, bool in, float bias,
-                                            int64_t out_row0) {
-  for (int c0 = half * kCols; c0 < x.rows; c0 += 2 * kCols) {
-    if (c0 + kCols <= x.rows) finish_columns<TO, ACT, true>(a, x, m, c0, tmem, in, bias, out_row0);
-    else finish_columns<TO, ACT, false>(a, x, m, c0, tmem, in, bias, out_row0);
+__device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int m, int part, uint32_t tmem, bool in, float bias,
+                                            int64_t out_row0, TO (&res)[kCols]) {
+  for (int c0 = part * kCols; c0 < x.rows; c0 += kEpiParts * kCols) {
+    uint32_t acc[kCols];
+    tmem_ld16(tmem + (uint32_t)c0, acc);
+    TO next[kCols];
+    const int c1 = c0 + kEpiParts * kCols;
+    if (a.r && in && c1 < x.rows) load_residual<TO>(a, out_row0 + c1, m, x.rows - c1, next);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    if (in) {
+      float v[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) v[c] = x.klen == 0 ? 0.f : __uint_as_float(acc[c]);  // an empty sum: no MMA wrote them
+      if (c0 + kCols <= x.rows) finish_values<TO, ACT, true>(a, out_row0 + c0, m, kCols, bias, res, v);
+      else finish_values<TO, ACT, false>(a, out_row0 + c0, m, x.rows - c0, bias, res, v);
+    }
+    if (a.r) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) res[c] = next[c];
+    }
     __syncwarp();  // tensor memory is read by the converged warp
   }
 }
 
-// Warp roles: 0 TMA producer, 1 MMA issuer, 2 clearing of ragged tails (kGradW), 4-11 epilogue.
+// Warp roles: 0 TMA producer, 1 MMA issuer, 2 clearing of ragged tails (kGradW), 4 and up epilogue.
 template <int KIND, typename TO>
 __global__ void __launch_bounds__(kMmThreads, 1)
 expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ MmArgs a) {
@@ -556,7 +558,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     }
   } else if (warp >= kEpiWarp0) {
     // ---------------- epilogue: lane = column of the output, accumulator column = row ----------------
-    const int quarter = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    const int quarter = warp & 3, part = (warp - kEpiWarp0) >> 2;
     int n = 0;
     for (int t = first; t < total && ok; t += stride, ++n) {
       const Tile x = tile_of<KIND>(t, a, s_off, s_tile, mblocks, jblocks);
@@ -564,18 +566,20 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const int m = x.m0 + (int)rank * kTileM + quarter * 32 + lane;
       const bool in = m < a.m_total;
       const float bias = a.bias && in ? load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type) : 0.f;
+      const int64_t out_row0 = KIND == kGradW ? (int64_t)x.e * a.j_total + x.row0 : (int64_t)x.row0;
+      TO res[kCols];
+      if (a.r && in && part * kCols < x.rows) load_residual<TO>(a, out_row0 + part * kCols, m, x.rows - part * kCols, res);
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * buf, (uint32_t)((n >> 1) & 1), limit))) {
         ok = false;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t d = tmem + (uint32_t)buf * kTileJ + ((uint32_t)(quarter * 32) << 16);
-      const int64_t out_row0 = KIND == kGradW ? (int64_t)x.e * a.j_total + x.row0 : (int64_t)x.row0;
       switch (KIND == kGradW ? ALPHASPARSE_ACT_NONE : a.act) {
-        case ALPHASPARSE_ACT_RELU: finish_tile<TO, ALPHASPARSE_ACT_RELU>(a, x, m, half, d, in, bias, out_row0); break;
-        case ALPHASPARSE_ACT_GELU: finish_tile<TO, ALPHASPARSE_ACT_GELU>(a, x, m, half, d, in, bias, out_row0); break;
-        case ALPHASPARSE_ACT_SILU: finish_tile<TO, ALPHASPARSE_ACT_SILU>(a, x, m, half, d, in, bias, out_row0); break;
-        default: finish_tile<TO, ALPHASPARSE_ACT_NONE>(a, x, m, half, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_RELU: finish_tile<TO, ALPHASPARSE_ACT_RELU>(a, x, m, part, d, in, bias, out_row0, res); break;
+        case ALPHASPARSE_ACT_GELU: finish_tile<TO, ALPHASPARSE_ACT_GELU>(a, x, m, part, d, in, bias, out_row0, res); break;
+        case ALPHASPARSE_ACT_SILU: finish_tile<TO, ALPHASPARSE_ACT_SILU>(a, x, m, part, d, in, bias, out_row0, res); break;
+        default: finish_tile<TO, ALPHASPARSE_ACT_NONE>(a, x, m, part, d, in, bias, out_row0, res); break;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       if (lane == 0) mbar_arrive(peer_u32(acc_empty + 8 * buf, 0));
