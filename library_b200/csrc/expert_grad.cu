@@ -1,11 +1,11 @@
 // Gradient of the experts' epilogue:  dZ = dY * act'(Z),  dBias[e] = column sums of the unrounded dZ over segment e.
 //
-// One pass over dY and Z.  A CTA takes a chunk of 256 rows x one stretch of columns and walks the
-// segments that meet the chunk; a segment's column sums stay in registers, are joined over the CTA's
-// warps through shared memory, and go to dBias at once when the segment lies inside the chunk, else
-// (a piece of it) to the workspace: slot 0 of the chunk for a segment that began earlier, slot 1 for
-// one that goes on.  A second kernel adds up the pieces of such segments in chunk order and
-// zeroes the rows of empty segments.  No atomics: the sums do not depend on the order of the CTAs.
+// One pass over dY and Z.  A CTA takes a chunk of 8 x R rows and a stretch of columns, each of its warps R consecutive rows: the warp
+// walks the segments that meet its rows with the column sums in registers.  A segment that lies inside the warp's rows goes to dBias
+// at once; the pieces at both ends of the warp's rows go to shared memory, where they are joined in warp order after one barrier, and
+// what reaches past the chunk goes to the workspace: slot 0 of the chunk for a segment that began before it, slot 1 for one that
+// goes on after it.  A second kernel adds up the pieces of such segments in chunk order and zeroes the rows of empty
+// segments.  No atomics: the sums do not depend on the order of the CTAs.
 #include "expert_act.h"
 #include "expert_launch.h"
 #include "expert_vec.h"
@@ -15,8 +15,7 @@ namespace {
 
 constexpr int kActThreads = 256;
 constexpr int kActWarps = kActThreads / 32;
-constexpr int kActRows = 256;
-constexpr int kActBatch = 4;
+constexpr int kActBatch = 4;  // rows in flight per warp
 
 __device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e, int segments, int rows) {
   if (!off) return e == 0 ? 0 : rows;
@@ -24,69 +23,123 @@ __device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e,
   return v < 0 ? 0 : v > rows ? rows : v;
 }
 
-template <typename T, int V, int ACT>
+// The last segment that begins at or before row r (0 if none does).  Whole warp.
+__device__ __forceinline__ int segment_of(const int32_t* __restrict__ off, int segments, int rows, int r) {
+  const int lane = threadIdx.x & 31, per = (segments + 31) / 32;
+  const unsigned hi = __ballot_sync(0xffffffffu, lane * per < segments && clamp_row(off, lane * per, segments, rows) <= r);
+  if (hi == 0) return 0;
+  const int blk = (31 - __clz(hi)) * per;
+  const unsigned lo = __ballot_sync(0xffffffffu, lane < per && blk + lane < segments && clamp_row(off, blk + lane, segments, rows) <= r);
+  return lo == 0 ? 0 : blk + 31 - __clz(lo);
+}
+
+template <typename T, int V, int U, int ACT>
 __global__ void __launch_bounds__(kActThreads, 3)
 expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz, int64_t lddz,
                        float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
-                       int cols, int strips, float* __restrict__ pieces) {
-  __shared__ float part[kActWarps][32 * V + 1];
+                       int cols, int strips, int warp_rows, float* __restrict__ pieces) {
+  constexpr int kStrip = 32 * V * U;
+  __shared__ float head[kActWarps][kStrip], tail[kActWarps][kStrip];
+  __shared__ int head_e[kActWarps], head_ends[kActWarps], tail_e[kActWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int chunk = (int)(blockIdx.x / (unsigned)strips), strip = (int)(blockIdx.x % (unsigned)strips);
-  const int r0 = chunk * kActRows, r1 = r0 < rows - kActRows ? r0 + kActRows : rows;
-  const int c0 = strip * 32 * V, c = c0 + lane * V;
+  const int chunk = (int)(blockIdx.x / (unsigned)strips), c_strip = (int)(blockIdx.x % (unsigned)strips) * kStrip;
   dependency_wait();
   dependents_go();
-  // the last segment that begins at or before the chunk
-  int before = 0;
-  for (int i = 0; i <= segments; i += kActThreads)
-    before += __syncthreads_count(i + tid <= segments && clamp_row(off, i + tid, segments, rows) <= r0);
-  for (int e = before > 0 ? before - 1 : 0; e < segments; ++e) {
+  const int64_t first = ((int64_t)chunk * kActWarps + warp) * warp_rows;
+  const int w0 = (int)(first < rows ? first : rows), w1 = (int)(first + warp_rows < rows ? first + warp_rows : rows);
+  int my_head = -1, my_ends = 0, my_tail = -1;
+  for (int r = w0, e = w0 < w1 ? segment_of(off, segments, rows, w0) : segments; r < w1 && e < segments; ++e) {
     const int b = clamp_row(off, e, segments, rows), d = clamp_row(off, e + 1, segments, rows);
-    if (b >= r1) break;
-    const int lo = b > r0 ? b : r0, hi = d < r1 ? d : r1;
+    if (b >= w1) break;
+    const int lo = b > r ? b : r, hi = d < w1 ? d : w1;
     if (lo >= hi) continue;
-    float sum[V];
+    float sum[U][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] = 0.f;
-    if (c < cols) {
-      // kActBatch rows are read before the first is written: dZ may be dY or Z, so the compiler cannot reorder them
-      for (int r = lo + warp; r < hi; r += kActWarps * kActBatch) {
-        Pack<T, V> g[kActBatch], a[kActBatch];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < kActBatch; ++i) {
-          const int row = r + i * kActWarps;
-          if (row >= hi) continue;
-          g[i] = load_pack<T, V>(dy + (int64_t)row * lddy + c);
-          if constexpr (ACT != ALPHASPARSE_ACT_NONE) a[i] = load_pack<T, V>(z + (int64_t)row * ldz + c);
+      for (int v = 0; v < V; ++v) sum[u][v] = 0.f;
+    // kActBatch rows are read before the first is written: dZ may be dY or Z, so the compiler cannot reorder them
+    for (int q = lo; q < hi; q += kActBatch) {
+      Pack<T, V> g[kActBatch][U], a[kActBatch][U];
+#pragma unroll
+      for (int i = 0; i < kActBatch; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c_strip + (32 * u + lane) * V;
+          if (q + i >= hi || c >= cols) continue;
+          g[i][u] = load_pack<T, V>(dy + (int64_t)(q + i) * lddy + c);
+          if constexpr (ACT != ALPHASPARSE_ACT_NONE) a[i][u] = load_pack<T, V>(z + (int64_t)(q + i) * ldz + c);
         }
 #pragma unroll
-        for (int i = 0; i < kActBatch; ++i) {
-          const int row = r + i * kActWarps;
-          if (row >= hi) continue;
+      for (int i = 0; i < kActBatch; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c_strip + (32 * u + lane) * V;
+          if (q + i >= hi || c >= cols) continue;
           float f[V];
 #pragma unroll
-          // (an explicit product: the sum below takes the same value whether or not dZ is stored)
+          // (an explicit product: the sum takes the same value whether or not dZ is stored)
           for (int v = 0; v < V; ++v) {
-            f[v] = g[i].at(v);
-            if constexpr (ACT != ALPHASPARSE_ACT_NONE) f[v] = __fmul_rn(f[v], act_slope<ACT>(a[i].at(v)));
-            sum[v] += f[v];
+            f[v] = g[i][u].at(v);
+            if constexpr (ACT != ALPHASPARSE_ACT_NONE) f[v] = __fmul_rn(f[v], act_slope<ACT>(a[i][u].at(v)));
+            sum[u][v] += f[v];
           }
-          if (dz) store_pack<T, V>(dz + (int64_t)row * lddz + c, round_pack<T, V>(f));
+          if (dz) store_pack<T, V>(dz + (int64_t)(q + i) * lddz + c, round_pack<T, V>(f));
+        }
+    }
+    r = hi;
+    if (!dbias) continue;
+    const bool before = b < w0, ends = hi == d;
+    float* out = before ? head[warp] : tail[warp];
+    if (before) {
+      my_head = e;
+      my_ends = ends;
+    } else if (!ends) {
+      my_tail = e;
+    } else {
+      out = nullptr;  // the whole segment
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = (32 * u + lane) * V + v;
+        if (out) out[i] = sum[u][v];
+        else if (c_strip + i < cols) dbias[(int64_t)e * lddb + c_strip + i] = sum[u][v];
+      }
+  }
+  if (!dbias) return;
+  if (lane == 0) {
+    head_e[warp] = my_head;
+    head_ends[warp] = my_ends;
+    tail_e[warp] = my_tail;
+  }
+  __syncthreads();
+  for (int i = tid; i < kStrip && c_strip + i < cols; i += kActThreads) {
+    float run = 0.f;
+    int open = -1;         // the segment that goes on into the next warp's rows
+    bool earlier = false;  // it began before the chunk
+    for (int w = 0; w < kActWarps; ++w) {
+      if (head_e[w] >= 0) {
+        if (open != head_e[w]) {
+          open = head_e[w];
+          earlier = true;
+          run = 0.f;
+        }
+        run += head[w][i];
+        if (head_ends[w]) {
+          if (earlier) pieces[(int64_t)(2 * chunk) * cols + c_strip + i] = run;
+          else dbias[(int64_t)open * lddb + c_strip + i] = run;
+          open = -1;
         }
       }
+      if (tail_e[w] >= 0) {
+        open = tail_e[w];
+        earlier = false;
+        run = tail[w][i];
+      }
     }
-    if (!dbias) continue;
-#pragma unroll
-    for (int v = 0; v < V; ++v) part[warp][lane * V + v] = sum[v];
-    __syncthreads();
-    float* out = b >= r0 && d <= r1 ? dbias + (int64_t)e * lddb : pieces + (int64_t)(2 * chunk + (b < r0 ? 0 : 1)) * cols;
-    for (int i = tid; i < 32 * V && c0 + i < cols; i += kActThreads) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kActWarps; ++w) s += part[w][i];
-      out[c0 + i] = s;
-    }
-    __syncthreads();
+    if (open >= 0) pieces[(int64_t)(2 * chunk + (earlier ? 0 : 1)) * cols + c_strip + i] = run;
   }
 }
 
@@ -94,20 +147,20 @@ expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz
 constexpr int kJoinCols = 64, kJoinParts = kActThreads / kJoinCols;
 __global__ void __launch_bounds__(kActThreads)
 expert_bias_join_kernel(float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
-                        int cols, int strips, const float* __restrict__ pieces) {
+                        int cols, int strips, int chunk_rows, const float* __restrict__ pieces) {
   __shared__ float part[kJoinParts][kJoinCols];
   dependency_wait();
   dependents_go();
   const int q = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
   const int e = (int)(blockIdx.x / (unsigned)strips), c = (int)(blockIdx.x % (unsigned)strips) * kJoinCols + i;
   const int b = clamp_row(off, e, segments, rows), d = clamp_row(off, e + 1, segments, rows);
-  const int k0 = b / kActRows, k1 = d > b ? (d - 1) / kActRows : k0;
+  const int k0 = b / chunk_rows, k1 = d > b ? (d - 1) / chunk_rows : k0;
   if (d > b && k0 == k1) return;  // written by the CTA of that chunk
   float sum = 0.f;
   if (d > b && c < cols) {
 #pragma unroll 8
     for (int k = k0 + q; k <= k1; k += kJoinParts)
-      sum += pieces[(int64_t)(2 * k + (b < k * kActRows ? 0 : 1)) * cols + c];
+      sum += pieces[(int64_t)(2 * k + ((int64_t)b < (int64_t)k * chunk_rows ? 0 : 1)) * cols + c];
   }
   part[q][i] = sum;
   __syncthreads();
@@ -119,52 +172,56 @@ expert_bias_join_kernel(float* __restrict__ dbias, int64_t lddb, const int32_t* 
   }
 }
 
+// Rows per warp: 32, fewer where that would leave some of the device's 148 SMs without a CTA.
+int act_warp_rows(int64_t rows, int64_t cols) {
+  int r = 32;
+  // (256 columns per CTA whatever the operands' alignment: the workspace's size may not depend on it)
+  while (r > 4 && (rows + kActWarps * r - 1) / (kActWarps * r) * ((cols + 255) / 256) < 148) r /= 2;
+  return r;
+}
 size_t piece_bytes(int64_t rows, int64_t cols) {
-  return (size_t)((rows + kActRows - 1) / kActRows) * 2 * (size_t)cols * sizeof(float) + 16;
+  const int64_t chunk = (int64_t)kActWarps * act_warp_rows(rows, cols);
+  return (size_t)((rows + chunk - 1) / chunk) * 2 * (size_t)cols * sizeof(float) + 16;
 }
 
 template <typename T, int V, int ACT>
 alphasparseStatus_t run_act_grad(alphasparseHandle_t h, int segments, const int32_t* off, alphasparseDnMatDescr_t dy,
                                  alphasparseDnMatDescr_t z, alphasparseDnMatDescr_t dz, alphasparseDnMatDescr_t db,
                                  void* buffer) {
-  const int rows = (int)dy->rows, cols = (int)dy->cols;
-  const int64_t chunks = ((int64_t)rows + kActRows - 1) / kActRows, strips = ((int64_t)cols + 32 * V - 1) / (32 * V);
+  constexpr int U = V == 1 ? 4 : V == 2 && sizeof(T) == 2 ? 2 : 1;
+  const int rows = (int)dy->rows, cols = (int)dy->cols, warp_rows = act_warp_rows(rows, cols), chunk_rows = kActWarps * warp_rows;
+  const int64_t chunks = ((int64_t)rows + chunk_rows - 1) / chunk_rows, strips = ((int64_t)cols + 32 * V * U - 1) / (32 * V * U);
   float* pieces = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(buffer) + 15) & ~(uintptr_t)15);
   if (chunks * strips >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
   if (chunks > 0) {
     const alphasparseStatus_t s = launch_chained(
-        h, expert_act_grad_kernel<T, V, ACT>, dim3((unsigned)(chunks * strips)), dim3(kActThreads), 0, 1, (const T*)dy->values, dy->ld,
+        h, expert_act_grad_kernel<T, V, U, ACT>, dim3((unsigned)(chunks * strips)), dim3(kActThreads), 0, 1, (const T*)dy->values, dy->ld,
         z ? (const T*)z->values : nullptr, z ? z->ld : 0, dz ? (T*)dz->values : nullptr, dz ? dz->ld : 0,
-        db ? (float*)db->values : nullptr, db ? db->ld : 0, off, segments, rows, cols, (int)strips, pieces);
+        db ? (float*)db->values : nullptr, db ? db->ld : 0, off, segments, rows, cols, (int)strips, warp_rows, pieces);
     if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   }
   if (!db) return ALPHA_SPARSE_STATUS_SUCCESS;
   const int64_t js = ((int64_t)cols + kJoinCols - 1) / kJoinCols;
   if (segments * js >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
   return launch_chained(h, expert_bias_join_kernel, dim3((unsigned)(segments * js)), dim3(kActThreads), 0, 1, (float*)db->values, db->ld,
-                        off, segments, rows, cols, (int)js, (const float*)pieces);
+                        off, segments, rows, cols, (int)js, chunk_rows, (const float*)pieces);
 }
 
 template <typename T>
 alphasparseStatus_t act_grad_t(alphasparseHandle_t h, int segments, const int32_t* off, alphasparseActivation_t act,
                                alphasparseDnMatDescr_t dy, alphasparseDnMatDescr_t z, alphasparseDnMatDescr_t dz,
                                alphasparseDnMatDescr_t db, void* buffer) {
-  constexpr int W = 16 / sizeof(T);
-  const bool wide = packs_of_16(dy) && packs_of_16(z) && packs_of_16(dz);
-  switch (act) {
-    case ALPHASPARSE_ACT_RELU:
-      return wide ? run_act_grad<T, W, ALPHASPARSE_ACT_RELU>(h, segments, off, dy, z, dz, db, buffer)
-                  : run_act_grad<T, 1, ALPHASPARSE_ACT_RELU>(h, segments, off, dy, z, dz, db, buffer);
-    case ALPHASPARSE_ACT_GELU:
-      return wide ? run_act_grad<T, W, ALPHASPARSE_ACT_GELU>(h, segments, off, dy, z, dz, db, buffer)
-                  : run_act_grad<T, 1, ALPHASPARSE_ACT_GELU>(h, segments, off, dy, z, dz, db, buffer);
-    case ALPHASPARSE_ACT_SILU:
-      return wide ? run_act_grad<T, W, ALPHASPARSE_ACT_SILU>(h, segments, off, dy, z, dz, db, buffer)
-                  : run_act_grad<T, 1, ALPHASPARSE_ACT_SILU>(h, segments, off, dy, z, dz, db, buffer);
-    default:
-      return wide ? run_act_grad<T, W, ALPHASPARSE_ACT_NONE>(h, segments, off, dy, z, dz, db, buffer)
-                  : run_act_grad<T, 1, ALPHASPARSE_ACT_NONE>(h, segments, off, dy, z, dz, db, buffer);
-  }
+  return by_pack<T>(
+      [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        switch (act) {
+          case ALPHASPARSE_ACT_RELU: return run_act_grad<T, V, ALPHASPARSE_ACT_RELU>(h, segments, off, dy, z, dz, db, buffer);
+          case ALPHASPARSE_ACT_GELU: return run_act_grad<T, V, ALPHASPARSE_ACT_GELU>(h, segments, off, dy, z, dz, db, buffer);
+          case ALPHASPARSE_ACT_SILU: return run_act_grad<T, V, ALPHASPARSE_ACT_SILU>(h, segments, off, dy, z, dz, db, buffer);
+          default: return run_act_grad<T, V, ALPHASPARSE_ACT_NONE>(h, segments, off, dy, z, dz, db, buffer);
+        }
+      },
+      dy, z, dz);
 }
 
 alphasparseStatus_t check_act_grad(alphasparseHandle_t h, int64_t segments, const int32_t* off,

@@ -861,16 +861,21 @@ struct Copy16 {
   uint16_t* out;
   int64_t rows, ld, ldo;
   int cols;
+  int64_t block;       // rows of an expert's block (0: all rows are wanted); those of experts without rows are left out
 };
 // Up to two matrices in one launch; a warp per row.
 __global__ void __launch_bounds__(256)
-expert_repack_kernel(const __grid_constant__ Copy16 a, const __grid_constant__ Copy16 b) {
+expert_repack_kernel(const __grid_constant__ Copy16 a, const __grid_constant__ Copy16 b, const int32_t* __restrict__ off, int rows) {
   dependency_wait();
   dependents_go();
   const int lane = threadIdx.x & 31;
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; i < a.rows + b.rows; i += (int64_t)gridDim.x * 8) {
     const Copy16& m = i < a.rows ? a : b;
     const int64_t r = i < a.rows ? i : i - a.rows;
+    if (m.block && off) {
+      const int e = (int)(r / m.block);
+      if (clamp_row(off, e, rows) >= clamp_row(off, e + 1, rows)) continue;
+    }
     const uint16_t* in = m.in + r * m.ld;
     uint16_t* out = m.out + r * m.ldo;
     constexpr int kBatch = 8;  // loads in flight
@@ -917,8 +922,9 @@ size_t repack_bytes(alphasparseDnMatDescr_t a, alphasparseDnMatDescr_t b) {
   const size_t n = repack_bytes(a) + repack_bytes(b);
   return n ? n + 256 : 0;
 }
-alphasparseStatus_t ready_operands(alphasparseHandle_t h, alphasparseDnMatDescr_t ma, alphasparseDnMatDescr_t mb, void* buffer, Operand* a,
-                                   Operand* b) {
+// (block: rows of an expert's block of mb, 0 if mb is not stacked)
+alphasparseStatus_t ready_operands(alphasparseHandle_t h, alphasparseDnMatDescr_t ma, alphasparseDnMatDescr_t mb, int64_t block,
+                                   const int32_t* off, void* buffer, Operand* a, Operand* b) {
   unsigned char* scratch = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(buffer) + 255) & ~(uintptr_t)255);
   Copy16 copies[2] = {};
   alphasparseDnMatDescr_t m[2] = {ma, mb};
@@ -928,12 +934,13 @@ alphasparseStatus_t ready_operands(alphasparseHandle_t h, alphasparseDnMatDescr_
     if (tma_ready(m[i])) continue;
     o[i]->p = scratch;
     o[i]->ld = padded8(m[i]->cols);
-    copies[i] = {(const uint16_t*)m[i]->values, (uint16_t*)o[i]->p, m[i]->rows, m[i]->ld, o[i]->ld, (int)m[i]->cols};
+    copies[i] = {(const uint16_t*)m[i]->values, (uint16_t*)o[i]->p, m[i]->rows, m[i]->ld, o[i]->ld, (int)m[i]->cols, i == 1 ? block : 0};
     scratch += repack_bytes(m[i]);
   }
   const int64_t blocks = (copies[0].rows + copies[1].rows + 7) / 8, most = 8 * (int64_t)impl(h)->sm_count;
   if (blocks == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
-  return launch_chained(h, expert_repack_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, 1, copies[0], copies[1]);
+  return launch_chained(h, expert_repack_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, 1, copies[0], copies[1],
+                        off, (int)ma->rows);
 }
 
 // blocks > 0: a third dimension over stacked blocks of rows / blocks rows each (out-of-range rows of a block read as
@@ -1013,13 +1020,14 @@ struct MmShape {
 };
 // Which kernel: 0 the pair kernel, else the one for few rows per segment with tiles of 16 (1) or 64 rows (2).  Up to 16 rows per
 // segment the weights' bytes are the work and many small CTAs draw them faster (64 experts x 2,048 x 1,408, 64 to 1,024 rows: 74-76 us
-// against 85-87; at 2,048 rows 89 against 87).  Beyond, up to 256 rows, it is the number of pair tiles that decides: a third of the
-// SMs' pairs or less leave the HBM idle (one 4,096 x 4,096 layer, 32 / 128 / 256 rows: 15 / 18 / 24 us against 26 / 28 / 29; 512 rows
-// 35 against 30; eight 2,048 x 2,048 layers, 256 rows: 23 against 22).
+// against 85-87; at 2,048 rows 89 against 87).  Beyond, it is the number of tiles that decides: where pair tiles would leave half of
+// the pairs idle and the small tiles still fit the device at once, the small ones run (one 4,096 x 4,096 layer, 32 / 128 / 256 rows:
+// 15 / 18 / 24 us against 26 / 28 / 29; 512 rows 35 against 30; eight 2,048 x 2,048 layers, 256 rows: 23 against 22).
 int few_rows(alphasparseHandle_t h, const MmShape& s, int64_t filled) {
   const int64_t pairs = (s.rows / kTileJ + filled) * ((s.n + kPairM - 1) / kPairM);
   if (s.rows <= 16 * filled) return 1;
-  return s.rows <= 256 * filled && pairs * 3 <= impl(h)->sm_count ? 2 : 0;
+  const int64_t small = (s.rows / 64 + filled) * ((s.n + kTileM - 1) / kTileM);
+  return pairs * 4 <= impl(h)->sm_count && small <= 2 * (int64_t)impl(h)->sm_count ? 2 : 0;
 }
 alphasparseStatus_t check_mm(alphasparseHandle_t h, alphasparseOperation_t op, int64_t segments, const int32_t* off,
                              alphasparseDnMatDescr_t x, alphasparseDnMatDescr_t w, alphasparseDnMatDescr_t y, MmShape* shape) {
@@ -1096,7 +1104,7 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   ASP_CUDA(dev.status);
   const bool nk = op == ALPHA_SPARSE_OPERATION_TRANSPOSE;
   Operand ox, ow;
-  if ((s = ready_operands(h, x, w, buffer, &ox, &ow)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  if ((s = ready_operands(h, x, w, nk ? shape.n : shape.k, off, buffer, &ox, &ow)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   MmArgs a = {};
   a.off = off;
   a.segments = (int)segments;
@@ -1156,7 +1164,7 @@ alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparse
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
   Operand om, oj;
-  if ((s = ready_operands(h, m, j, buffer, &om, &oj)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
+  if ((s = ready_operands(h, m, j, 0, nullptr, buffer, &om, &oj)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   MmArgs a = {};
   a.off = off;
   a.segments = (int)segments;

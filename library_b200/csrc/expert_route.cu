@@ -378,7 +378,7 @@ __device__ __forceinline__ float reduce_values(float (&v)[J], int lane) {
 // and four CTAs per SM take 81 us; one token per CTA 90 us; eight rows in flight (three CTAs fit) 105 us, without a register limit
 // (one CTA) 189 us.
 constexpr int kGradThreads = 128;  // of a token
-template <typename T, int V, int J>
+template <typename T, int V, int U, int J>
 __global__ void __launch_bounds__(kRowThreads, 4)
 route_combine_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* ys, int64_t ldys,
                           const float* __restrict__ weights, T* dys, int64_t lddys, float* __restrict__ dweights,
@@ -402,31 +402,43 @@ route_combine_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* ys, i
     for (int i = 0; i < J; ++i) dot[i] = 0.f;
     if (t < tokens) {
       // (whole warps step together: the shuffles below need every lane)
-      for (int c0 = (int)threadIdx.x - lane; c0 < packs; c0 += (int)blockDim.x) {
-        const int c = c0 + lane;
-        const bool in_row = c < packs;
-        Pack<T, V> g, in[J];
-        if (in_row) g = load_pack<T, V>(dy + (int64_t)t * lddy + (int64_t)c * V);
+      for (int c0 = (int)threadIdx.x - lane; c0 < packs; c0 += (int)blockDim.x * U) {
+        Pack<T, V> g[U], in[J][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + lane + (int)blockDim.x * u;
+          if (c < packs) g[u] = load_pack<T, V>(dy + (int64_t)t * lddy + (int64_t)c * V);
+        }
         if (dweights) {
 #pragma unroll
           for (int i = 0; i < J; ++i) {
             const int p = __shfl_sync(0xffffffffu, p_mine, i);
-            if (in_row && (unsigned)p < (unsigned)rows) in[i] = load_pack<T, V>(ys + (int64_t)p * ldys + (int64_t)c * V);
+            if ((unsigned)p >= (unsigned)rows) continue;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int c = c0 + lane + (int)blockDim.x * u;
+              if (c < packs) in[i][u] = load_pack<T, V>(ys + (int64_t)p * ldys + (int64_t)c * V);
+            }
           }
         }
 #pragma unroll
         for (int i = 0; i < J; ++i) {
           const int p = __shfl_sync(0xffffffffu, p_mine, i);
           const float w = __shfl_sync(0xffffffffu, w_mine, i);
-          if (!in_row || (unsigned)p >= (unsigned)rows) continue;
-          float out[V];
+          if ((unsigned)p >= (unsigned)rows) continue;
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float gv = g.at(v);
-            if (dweights) dot[i] = fmaf(gv, in[i].at(v), dot[i]);
-            out[v] = w * gv;
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + lane + (int)blockDim.x * u;
+            if (c >= packs) continue;
+            float out[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              const float gv = g[u].at(v);
+              if (dweights) dot[i] = fmaf(gv, in[i][u].at(v), dot[i]);
+              out[v] = w * gv;
+            }
+            if (dys) store_pack<T, V>(dys + (int64_t)p * lddys + (int64_t)c * V, round_pack<T, V>(out));
           }
-          if (dys) store_pack<T, V>(dys + (int64_t)p * lddys + (int64_t)c * V, round_pack<T, V>(out));
         }
         __syncwarp();
       }
@@ -501,7 +513,7 @@ int64_t row_blocks(int64_t tokens, int64_t stretches) { return (tokens * stretch
 template <typename T, int V>
 alphasparseStatus_t run_dispatch(alphasparseHandle_t h, alphasparseRoutingDescr_t r, alphasparseDnMatDescr_t x,
                                  alphasparseDnMatDescr_t xs) {
-  constexpr int U = 4;
+  constexpr int U = packs_per_lane<T, V>(64);
   const int64_t packs = x->cols / V, stretches = (packs + 32 * U - 1) / (32 * U);
   const int64_t blocks = row_blocks(r->tokens, stretches);
   if (blocks >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
@@ -513,7 +525,7 @@ alphasparseStatus_t run_dispatch(alphasparseHandle_t h, alphasparseRoutingDescr_
 template <typename T, int V>
 alphasparseStatus_t run_combine(alphasparseHandle_t h, alphasparseRoutingDescr_t r, alphasparseDnMatDescr_t ys,
                                 const float* weights, alphasparseDnMatDescr_t res, alphasparseDnMatDescr_t y) {
-  constexpr int U = V == 1 ? 8 : 2;
+  constexpr int U = packs_per_lane<T, V>(32);
   const int64_t packs = y->cols / V, stretches = (packs + 32 * U - 1) / (32 * U);
   const int64_t blocks = row_blocks(r->tokens, stretches);
   if (blocks >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
@@ -528,10 +540,11 @@ alphasparseStatus_t run_combine_grad(alphasparseHandle_t h, alphasparseRoutingDe
                                      float* dweights, int64_t rows) {
   const int64_t packs = dy->cols / V;
   int x = 32;
-  while (x < kGradThreads && x < packs) x *= 2;
+  constexpr int U = packs_per_lane<T, V>(16);
+  while (x < kGradThreads && (int64_t)x * U < packs) x *= 2;
   const int y = kRowThreads / x;
   const int64_t blocks = (r->tokens + y - 1) / y;
-  return launch_chained(h, route_combine_grad_kernel<T, V, 4>, dim3((unsigned)blocks), dim3(x, y), 0, 1,
+  return launch_chained(h, route_combine_grad_kernel<T, V, U, 4>, dim3((unsigned)blocks), dim3(x, y), 0, 1,
       (const T*)dy->values, dy->ld, ys ? (const T*)ys->values : nullptr, ys ? ys->ld : 0, weights,
       dys ? (T*)dys->values : nullptr, dys ? dys->ld : 0, dweights, r->position, (int)r->tokens, (int)r->topk, (int)packs,
       (int)rows);
@@ -573,10 +586,9 @@ alphasparseStatus_t alphasparseRoutingDispatch(alphasparseHandle_t h, alphaspars
   if (r->tokens == 0 || x->cols == 0 || xs->rows == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
-  const bool wide = packs_of_16(x) && packs_of_16(xs);
   return by_type(x->data_type, [&](auto t) {
     using T = decltype(t);
-    return wide ? run_dispatch<T, 16 / sizeof(T)>(h, r, x, xs) : run_dispatch<T, 1>(h, r, x, xs);
+    return by_pack<T>([&](auto v) { return run_dispatch<T, decltype(v)::value>(h, r, x, xs); }, x, xs);
   });
 }
 
@@ -594,10 +606,9 @@ alphasparseStatus_t alphasparseRoutingCombine(alphasparseHandle_t h, alphasparse
   if (r->tokens == 0 || y->cols == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
-  const bool wide = packs_of_16(ys) && packs_of_16(res) && packs_of_16(y);
   return by_type(y->data_type, [&](auto t) {
     using T = decltype(t);
-    return wide ? run_combine<T, 16 / sizeof(T)>(h, r, ys, weights, res, y) : run_combine<T, 1>(h, r, ys, weights, res, y);
+    return by_pack<T>([&](auto v) { return run_combine<T, decltype(v)::value>(h, r, ys, weights, res, y); }, ys, res, y);
   });
 }
 
@@ -616,11 +627,10 @@ alphasparseStatus_t alphasparseRoutingCombineGrad(alphasparseHandle_t h, alphasp
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
   const int64_t rows = dys ? dys->rows : ys->rows;
-  const bool wide = packs_of_16(dy) && packs_of_16(ys) && packs_of_16(dys);
   return by_type(dy->data_type, [&](auto t) {
     using T = decltype(t);
-    return wide ? run_combine_grad<T, 16 / sizeof(T)>(h, r, dy, ys, weights, dys, dweights, rows)
-                : run_combine_grad<T, 1>(h, r, dy, ys, weights, dys, dweights, rows);
+    return by_pack<T>([&](auto v) { return run_combine_grad<T, decltype(v)::value>(h, r, dy, ys, weights, dys, dweights, rows); }, dy,
+                      ys, dys);
   });
 }
 
