@@ -55,6 +55,11 @@ __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The arrival that hands an accumulator back: its reads have completed (tcgen05.wait::ld), nothing else has to be visible.  A release
+// at cluster scope would wait for the epilogue's global stores.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Bounded wait on a barrier of this CTA: false if the phase did not complete within `limit` polls.  A poll parks the warp for up to two
 // microseconds or until the phase completes: a warp that polls flat out costs power, and power is what limits the products.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
@@ -313,7 +318,7 @@ __device__ __forceinline__ Tile tile_of(int t, const MmArgs& a, const int* s_off
   return x;
 }
 
-constexpr int kCols = 16;  // (32 at a time spilled registers)
+constexpr int kCols = 16;  // (32 at a time spilled registers; 8 take a third longer)
 // The epilogue of kCols rows (n of them exist, all if FULL) of output column m, from row `row` of the output on: v holds the
 // sums.  Each optional operand is one guarded loop, not a test per element.
 template <typename TO>
@@ -346,28 +351,22 @@ __device__ __forceinline__ void finish_values(const MmArgs& a, int64_t row, int 
   for (int c = 0; c < kCols; ++c, y += a.ldy)
     if (FULL || c < n) *y = Wide<TO>::down(v[c]);
 }
-// A warp's share of a tile: every kEpiParts-th block of kCols rows.  res holds the residual of the first; that of the next block is
-// asked for before a block is finished, so that its latency passes behind the block's arithmetic.
-template <typename TO, int ACT>
+// A warp's share of a tile: every PARTS-th block of kCols rows.
+template <typename TO, int ACT, int PARTS = kEpiParts>
 __device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int m, int part, uint32_t tmem, bool in, float bias,
-                                            int64_t out_row0, TO (&res)[kCols]) {
-  for (int c0 = part * kCols; c0 < x.rows; c0 += kEpiParts * kCols) {
+                                            int64_t out_row0) {
+  for (int c0 = part * kCols; c0 < x.rows; c0 += PARTS * kCols) {
+    TO res[kCols];
+    if (a.r && in) load_residual<TO>(a, out_row0 + c0, m, x.rows - c0, res);
     uint32_t acc[kCols];
     tmem_ld16(tmem + (uint32_t)c0, acc);
-    TO next[kCols];
-    const int c1 = c0 + kEpiParts * kCols;
-    if (a.r && in && c1 < x.rows) load_residual<TO>(a, out_row0 + c1, m, x.rows - c1, next);
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     if (in) {
       float v[kCols];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) v[c] = x.klen == 0 ? 0.f : __uint_as_float(acc[c]);  // an empty sum: no MMA wrote them
+      for (int c = 0; c < kCols; ++c) v[c] = x.klen <= 0 ? 0.f : __uint_as_float(acc[c]);  // an empty sum: no MMA wrote them
       if (c0 + kCols <= x.rows) finish_values<TO, ACT, true>(a, out_row0 + c0, m, kCols, bias, res, v);
       else finish_values<TO, ACT, false>(a, out_row0 + c0, m, x.rows - c0, bias, res, v);
-    }
-    if (a.r) {
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) res[c] = next[c];
     }
     __syncwarp();  // tensor memory is read by the converged warp
   }
@@ -567,8 +566,13 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const bool in = m < a.m_total;
       const float bias = a.bias && in ? load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type) : 0.f;
       const int64_t out_row0 = KIND == kGradW ? (int64_t)x.e * a.j_total + x.row0 : (int64_t)x.row0;
-      TO res[kCols];
-      if (a.r && in && part * kCols < x.rows) load_residual<TO>(a, out_row0 + part * kCols, m, x.rows - part * kCols, res);
+      if (a.r) {
+        // the tile's residual on its way to L2 while the accumulator is still being formed: a row per lane of the epilogue
+        const int row = (warp - kEpiWarp0) * 32 + lane, m_cta = x.m0 + (int)rank * kTileM;
+        const TO* r = (const TO*)a.r + (out_row0 + row) * a.ldr + m_cta;
+        for (int c = 0; row < x.rows && c < kTileM && m_cta + c < a.m_total; c += 128 / (int)sizeof(TO))
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(r + c));
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full + 8 * buf, (uint32_t)((n >> 1) & 1), limit))) {
         ok = false;
         break;
@@ -576,13 +580,13 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t d = tmem + (uint32_t)buf * kTileJ + ((uint32_t)(quarter * 32) << 16);
       switch (KIND == kGradW ? ALPHASPARSE_ACT_NONE : a.act) {
-        case ALPHASPARSE_ACT_RELU: finish_tile<TO, ALPHASPARSE_ACT_RELU>(a, x, m, part, d, in, bias, out_row0, res); break;
-        case ALPHASPARSE_ACT_GELU: finish_tile<TO, ALPHASPARSE_ACT_GELU>(a, x, m, part, d, in, bias, out_row0, res); break;
-        case ALPHASPARSE_ACT_SILU: finish_tile<TO, ALPHASPARSE_ACT_SILU>(a, x, m, part, d, in, bias, out_row0, res); break;
-        default: finish_tile<TO, ALPHASPARSE_ACT_NONE>(a, x, m, part, d, in, bias, out_row0, res); break;
+        case ALPHASPARSE_ACT_RELU: finish_tile<TO, ALPHASPARSE_ACT_RELU>(a, x, m, part, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_GELU: finish_tile<TO, ALPHASPARSE_ACT_GELU>(a, x, m, part, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_SILU: finish_tile<TO, ALPHASPARSE_ACT_SILU>(a, x, m, part, d, in, bias, out_row0); break;
+        default: finish_tile<TO, ALPHASPARSE_ACT_NONE>(a, x, m, part, d, in, bias, out_row0); break;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      if (lane == 0) mbar_arrive(peer_u32(acc_empty + 8 * buf, 0));
+      if (lane == 0) mbar_arrive_relaxed(peer_u32(acc_empty + 8 * buf, 0));
     }
   }
   __syncwarp();
@@ -600,6 +604,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 }
 
 // ---- few rows: the weights' bytes are the work ----------------------------------------------------
+// (and, for gradients, few tiles: a long contraction would run on few SMs).
 // One output tile of 128 columns x up to J rows per CLUSTER, whose CTAs share the contraction: each streams its
 // part of K through a ring of its own (several CTAs per SM, so that many loads are in flight),
 // leaves its fp32 sums in shared memory, and after a cluster barrier CTA r adds up the rows r, r + size, ... over all
@@ -672,8 +677,8 @@ __device__ __forceinline__ float ld_peer(uint32_t addr) {
 }
 
 template <typename TO, int ACT>
-__device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, int m, int col, uint32_t sums, uint32_t rank, uint32_t size,
-                                              bool in, float bias) {
+__device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, int64_t row0, int m, int col, uint32_t sums, uint32_t rank,
+                                              uint32_t size, bool in, float bias) {
   // four rows at a time, their partial sums of all CTAs in flight together
   for (int j0 = (int)rank; j0 < x.rows; j0 += (int)size * 4) {
     float v[4];
@@ -685,7 +690,7 @@ __device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, in
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = j0 + i * (int)size;
-        if (j < x.rows) res[i] = ((const TO*)a.r)[(int64_t)(x.row0 + j) * a.ldr + m];
+        if (j < x.rows) res[i] = ((const TO*)a.r)[(row0 + j) * a.ldr + m];
       }
     }
     for (uint32_t c = 0; c < size; ++c) {
@@ -700,7 +705,7 @@ __device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, in
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + i * (int)size;
       if (j >= x.rows) continue;
-      const int64_t row = x.row0 + j;
+      const int64_t row = row0 + j;
       float w = v[i] + bias;
       if (a.z) ((TO*)a.z)[row * a.ldz + m] = Wide<TO>::down(w);
       w = activate<ACT>(w);
@@ -747,17 +752,32 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   dependents_go();  // tensor memory is allocated
   dependency_wait();
   Tile x;
-  if (!few_tile<J>(t / mblocks, a, x)) {  // the whole cluster: the grid covers the most tiles these sizes can have
-    if (warp == 1) tmem_free<1>(tmem, kFewTmem);
-    return;
+  int64_t out_row0;
+  if constexpr (KIND == kGradW) {
+    const int per = mblocks * ((a.j_total + J - 1) / J);
+    x.e = t / per;
+    x.row0 = t % per / mblocks * J;
+    x.rows = a.j_total - x.row0 < J ? a.j_total - x.row0 : J;
+    x.width = (x.rows + 15) & ~15;
+    x.k0 = a.off ? clamp_row(a.off, x.e, a.rows) : 0;
+    x.klen = (a.off ? clamp_row(a.off, x.e + 1, a.rows) : a.rows) - x.k0;
+    out_row0 = (int64_t)x.e * a.j_total + x.row0;
+  } else {
+    if (!few_tile<J>(t / mblocks, a, x)) {  // the whole cluster: the grid covers the most tiles these sizes can have
+      if (warp == 1) tmem_free<1>(tmem, kFewTmem);
+      return;
+    }
+    x.k0 = 0;
+    x.klen = a.k;
+    out_row0 = x.row0;
   }
   x.m0 = (t % mblocks) * kTileM;
-  const int chunks = (a.k + kKC - 1) / kKC;
+  const int chunks = x.klen > 0 ? (x.klen + kKC - 1) / kKC : 0;
   const int c0 = (int)((int64_t)chunks * rank / size), c1 = (int)((int64_t)chunks * (rank + 1) / size);
   bool ok = true;
   if (warp == 0) {
-    const int boxes = x.width / kFewBox;
-    const uint32_t bytes = kABytes + (uint32_t)(boxes * kFewBox * 128);
+    const int boxes = KIND == kGradW ? 0 : x.width / kFewBox;
+    const uint32_t bytes = kABytes + (uint32_t)(KIND == kGradW ? kBoxBytes : boxes * kFewBox * 128);
     int st = 0;
     uint32_t ph = 0;
     for (int c = c0; c < c1; ++c) {
@@ -772,10 +792,14 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
           // testing, as in the kernel above
         } else if constexpr (KIND == kFwdT) {
           tma_3d<1>(sa, &map_a, c * kKC, x.m0, x.e, bar);
+        } else if constexpr (KIND == kGradW) {
+          tma_2d<1>(sa, &map_a, x.m0, x.k0 + c * kKC, bar);
+          tma_2d<1>(sa + kBoxBytes, &map_a, x.m0 + 64, x.k0 + c * kKC, bar);
         } else {
           tma_3d<1>(sa, &map_a, x.m0, c * kKC, x.e, bar);
           tma_3d<1>(sa + kBoxBytes, &map_a, x.m0 + 64, c * kKC, x.e, bar);
         }
+        if constexpr (KIND == kGradW) tma_2d<1>(sb, &map_b, x.row0, x.k0 + c * kKC, bar);
         for (int b = 0; b < boxes; ++b) tma_2d<1>(sb + b * kFewBox * 128, &map_b, c * kKC, x.row0 + b * kFewBox, bar);
       }
       __syncwarp();
@@ -787,19 +811,29 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   } else if (warp == 1) {
     int st = 0;
     uint32_t ph = 0;
-    constexpr uint32_t kMajor = KIND == kFwdN ? (1u << 15) : 0u;
+    constexpr uint32_t kMajor = KIND == kFwdN ? (1u << 15) : KIND == kGradW ? (1u << 15) | (1u << 16) : 0u;
     const uint32_t idesc = (1u << 4) | a.types | kMajor | ((uint32_t)(x.width >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
-    constexpr uint32_t kStepA = KIND == kFwdT ? 2u : 128u;
+    constexpr uint32_t kStepA = KIND == kFwdT ? 2u : 128u, kStepB = KIND == kGradW ? 128u : 2u;
     for (int c = c0; c < c1; ++c) {
       if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, ph, limit))) {
         ok = false;
         break;
       }
+      const int left = x.klen - c * kKC;
+      if (KIND == kGradW && left < kKC && (left & 15) != 0) {
+        // rows of the next segment (or none) behind the last one: zeros up to the MMA's sixteen
+        const int n16 = (((left + 15) & ~15) - left) * 8;
+        unsigned char* tile = gen + st * kStage;
+        for (int i = lane; i < 3 * n16; i += 32)  // whole rows of 128 bytes: the swizzle does not matter
+          *reinterpret_cast<uint4*>(tile + (i / n16) * kBoxBytes + left * 128 + (i % n16) * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (elect_one()) {
         const uint64_t da = umma_desc(base + st * kStage, kBoxBytes), db = umma_desc(base + st * kStage + kABytes, kBoxBytes);
-        const int left = a.k - c * kKC, steps = left >= kKC ? kKC / 16 : (left + 15) / 16;
-        for (int s = 0; s < steps; ++s) umma<1>(tmem, da + s * kStepA, db + s * 2u, idesc, c > c0 || s > 0 ? 1u : 0u);
+        const int steps = left >= kKC ? kKC / 16 : (left + 15) / 16;
+        for (int s = 0; s < steps; ++s) umma<1>(tmem, da + s * kStepA, db + s * kStepB, idesc, c > c0 || s > 0 ? 1u : 0u);
         umma_commit<1>(empty + 8 * st);
       }
       __syncwarp();
@@ -819,7 +853,15 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (a.bias && in) bias = load_bias(a.bias, (int64_t)x.e * a.ldb + m, a.bias_type);
     ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0u, limit));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (ok) {
+    if (ok && size == 1) {
+      const uint32_t d = tmem + ((uint32_t)(quarter * 32) << 16);
+      switch (KIND == kGradW ? (int)ALPHASPARSE_ACT_NONE : a.act) {
+        case ALPHASPARSE_ACT_RELU: finish_tile<TO, ALPHASPARSE_ACT_RELU, 1>(a, x, m, 0, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_GELU: finish_tile<TO, ALPHASPARSE_ACT_GELU, 1>(a, x, m, 0, d, in, bias, out_row0); break;
+        case ALPHASPARSE_ACT_SILU: finish_tile<TO, ALPHASPARSE_ACT_SILU, 1>(a, x, m, 0, d, in, bias, out_row0); break;
+        default: finish_tile<TO, ALPHASPARSE_ACT_NONE, 1>(a, x, m, 0, d, in, bias, out_row0); break;
+      }
+    } else if (ok) {
       // every MMA of this CTA is done: the ring's memory takes the sums, [row][column]
       float* sums = reinterpret_cast<float*>(gen);
       for (int j0 = 0; j0 < x.rows; j0 += kCols) {
@@ -841,12 +883,12 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   }
   if (size > 1) cluster_sync();  // the peers' sums are complete
-  if (epilogue && !*s_fail) {
-    switch (a.act) {
-      case ALPHASPARSE_ACT_RELU: finish_shared<TO, ALPHASPARSE_ACT_RELU>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
-      case ALPHASPARSE_ACT_GELU: finish_shared<TO, ALPHASPARSE_ACT_GELU>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
-      case ALPHASPARSE_ACT_SILU: finish_shared<TO, ALPHASPARSE_ACT_SILU>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
-      default: finish_shared<TO, ALPHASPARSE_ACT_NONE>(a, x, m, col, base, rank, (uint32_t)size, in, bias); break;
+  if (epilogue && size > 1 && !*s_fail) {
+    switch (KIND == kGradW ? (int)ALPHASPARSE_ACT_NONE : a.act) {
+      case ALPHASPARSE_ACT_RELU: finish_shared<TO, ALPHASPARSE_ACT_RELU>(a, x, out_row0, m, col, base, rank, (uint32_t)size, in, bias); break;
+      case ALPHASPARSE_ACT_GELU: finish_shared<TO, ALPHASPARSE_ACT_GELU>(a, x, out_row0, m, col, base, rank, (uint32_t)size, in, bias); break;
+      case ALPHASPARSE_ACT_SILU: finish_shared<TO, ALPHASPARSE_ACT_SILU>(a, x, out_row0, m, col, base, rank, (uint32_t)size, in, bias); break;
+      default: finish_shared<TO, ALPHASPARSE_ACT_NONE>(a, x, out_row0, m, col, base, rank, (uint32_t)size, in, bias); break;
     }
   }
   __syncwarp();
@@ -992,24 +1034,25 @@ alphasparseStatus_t launch_mm(alphasparseHandle_t h, const CUtensorMap& ma, cons
 }
 
 template <int KIND, int J, typename TO>
-alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles) {
+alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
+                               int64_t chunks) {
   static std::atomic<uint64_t> done{0};
   const auto kernel = expert_mm_few_kernel<KIND, J, TO>;
   const alphasparseStatus_t s = allow_smem(kernel, Few<J>::kSmem, h->device, &done);
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   // CTAs that share a tile's contraction: as many as fit the device at once, a ring's worth of stages each
-  const int chunks = (a.k + kKC - 1) / kKC, resident = (J == 16 ? 3 : 2) * impl(h)->sm_count;
+  const int resident = (J == 16 ? 3 : 2) * impl(h)->sm_count;
   int size = 1;
   while (size < 8 && tiles * size * 2 <= resident && chunks >= 2 * size * kFewStages) size *= 2;
   return launch_chained(h, kernel, dim3((unsigned)(tiles * size)), dim3(kFewThreads), Few<J>::kSmem, size, ma, mb, a, size);
 }
 template <int KIND, int J>
 alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
-                               alphasparseDataType out) {
+                               int64_t chunks, alphasparseDataType out) {
   switch (out) {
-    case ALPHA_R_32F: return launch_few<KIND, J, float>(h, ma, mb, a, tiles);
-    case ALPHA_R_16F: return launch_few<KIND, J, __half>(h, ma, mb, a, tiles);
-    default: return launch_few<KIND, J, __nv_bfloat16>(h, ma, mb, a, tiles);
+    case ALPHA_R_32F: return launch_few<KIND, J, float>(h, ma, mb, a, tiles, chunks);
+    case ALPHA_R_16F: return launch_few<KIND, J, __half>(h, ma, mb, a, tiles, chunks);
+    default: return launch_few<KIND, J, __nv_bfloat16>(h, ma, mb, a, tiles, chunks);
   }
 }
 
@@ -1132,10 +1175,11 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   }
   if (few) {
     const int j = few == 1 ? 16 : 64;
+    const int64_t chunks = (shape.k + kKC - 1) / kKC;
     const int64_t tiles = (shape.rows / j + filled) * ((shape.n + kTileM - 1) / kTileM);
     if (few == 1)
-      return nk ? launch_few<kFwdT, 16>(h, mw, mx, a, tiles, y->data_type) : launch_few<kFwdN, 16>(h, mw, mx, a, tiles, y->data_type);
-    return nk ? launch_few<kFwdT, 64>(h, mw, mx, a, tiles, y->data_type) : launch_few<kFwdN, 64>(h, mw, mx, a, tiles, y->data_type);
+      return nk ? launch_few<kFwdT, 16>(h, mw, mx, a, tiles, chunks, y->data_type) : launch_few<kFwdN, 16>(h, mw, mx, a, tiles, chunks, y->data_type);
+    return nk ? launch_few<kFwdT, 64>(h, mw, mx, a, tiles, chunks, y->data_type) : launch_few<kFwdN, 64>(h, mw, mx, a, tiles, chunks, y->data_type);
   }
   const int64_t tiles = (shape.rows / kTileJ + filled) * ((shape.n + kPairM - 1) / kPairM);
   return nk ? launch_mm<kFwdT>(h, mw, mx, a, tiles, y->data_type) : launch_mm<kFwdN>(h, mw, mx, a, tiles, y->data_type);
@@ -1183,6 +1227,11 @@ alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparse
   }
   const int64_t tiles = segments * ((m->cols + kPairM - 1) / kPairM) * ((j->cols + kTileJ - 1) / kTileJ);
   if (tiles >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
+  // as in few_rows: small tiles, and clusters that share the rows of a segment, where pair tiles would leave half of the pairs idle and
+  // the contraction is long (two segments, 3,879 rows, 432 x 232: 24 us with dX against 32; below 512 rows a segment it loses 2 us)
+  const int64_t small = segments * ((m->cols + kTileM - 1) / kTileM) * ((j->cols + 63) / 64);
+  if (x->rows > 512 * segments && tiles * 4 <= impl(h)->sm_count && small <= 2 * (int64_t)impl(h)->sm_count)
+    return launch_few<kGradW, 64>(h, mm, mj, a, small, x->rows / (segments * kKC), dw->data_type);
   return launch_mm<kGradW>(h, mm, mj, a, tiles, dw->data_type);
 }
 
