@@ -296,7 +296,7 @@ def routed(tokens, topk, experts, seed, dropped=0.2):
 
 
 SHAPES = [(1, 1, 1, 0, 0), (1, 8, 4096, 0, 0), (5, 2, 64, 8, 8), (37, 3, 1003, 0, 0), (37, 3, 1000, 24, 0), (64, 33, 7, 5, 3),
-          (300, 8, 520, 8, 1), (129, 6, 2048, 0, 0), (2, 64, 40, 0, 0), (3, 4, 20000, 0, 0)]
+          (300, 8, 520, 8, 1), (129, 6, 2048, 0, 0), (2, 64, 40, 0, 0), (3, 4, 20000, 0, 0), (50, 3, 1258, 0, 0), (41, 2, 90, 2, 2)]
 
 
 @pytest.mark.gpu
@@ -390,11 +390,12 @@ def test_dispatch_passes_over_bad_positions(h):
 
 # counts per segment, K, N: one row; one token's choice of experts; ragged with empty segments at both ends; a plain dense
 # layer; tiles cut in every direction; K from nothing up; many segments, as many as there may be; nothing but empty ones; more tiles
-# than the device holds at once; both kernels for few rows, with and without a shared contraction
+# than the device holds at once; both kernels for few rows, with and without a shared contraction; long segments of small products
 PRODUCTS = [([1], 64, 64), ([0, 1, 0, 1, 1], 256, 200), ([0, 130, 1, 0, 257, 64, 0], 192, 136), ([300], 512, 384), ([17], 1024, 640),
             ([5, 9], 8, 8), ([3, 0, 2], 1, 1), ([70, 3], 0, 24), ([33, 40], 1000, 515), ([129, 255, 256], 72, 264),
             ([2] * 200 + [0] * 100 + [3] * 57, 40, 24), ([600, 1], 2048, 128), ([0, 0, 0], 64, 40), ([20] * 1023 + [40], 24, 16),
-            ([10] * 33, 136, 72), ([700, 900, 257, 0, 1200], 320, 2000), ([64, 50, 1], 1096, 3000), ([48] * 40, 128, 1032)]
+            ([10] * 33, 136, 72), ([700, 900, 257, 0, 1200], 320, 2000), ([64, 50, 1], 1096, 3000), ([48] * 40, 128, 1032),
+            ([1100], 200, 136), ([1300, 0, 900], 72, 40)]
 
 
 def product_inputs(counts, k, n, op, dt, seed, pad, shift, tail):
@@ -416,7 +417,7 @@ def product_inputs(counts, k, n, op, dt, seed, pad, shift, tail):
 @pytest.mark.gpu
 @pytest.mark.parametrize("op", [api.OP_T, api.OP_N])
 @pytest.mark.parametrize("case", range(len(PRODUCTS)))
-@pytest.mark.parametrize("dt,pad,shift", [(torch.bfloat16, 0, 0), (torch.float16, 8, 8), (torch.bfloat16, 3, 1)])
+@pytest.mark.parametrize("dt,pad,shift", [(torch.bfloat16, 0, 0), (torch.float16, 8, 8), (torch.bfloat16, 3, 1), (torch.float16, 2, 2)])
 def test_expert_mm(h, case, op, dt, pad, shift):
     counts, k, n = PRODUCTS[case]
     tail = 5 if case % 2 == 0 and case else 0
@@ -467,7 +468,7 @@ def test_expert_mm(h, case, op, dt, pad, shift):
 @pytest.mark.gpu
 @pytest.mark.parametrize("op", [api.OP_T, api.OP_N])
 @pytest.mark.parametrize("case", range(len(PRODUCTS)))
-@pytest.mark.parametrize("dt,pad,shift", [(torch.bfloat16, 0, 0), (torch.float16, 8, 8), (torch.bfloat16, 3, 1)])
+@pytest.mark.parametrize("dt,pad,shift", [(torch.bfloat16, 0, 0), (torch.float16, 8, 8), (torch.bfloat16, 3, 1), (torch.float16, 2, 2)])
 def test_expert_mm_grad_weight(h, case, op, dt, pad, shift):
     counts, k, n = PRODUCTS[case]
     tail = 5 if case % 2 == 0 and case else 0
@@ -582,7 +583,8 @@ def test_waits_that_run_out_are_reported(monkeypatch):
 # ---- the epilogue's gradient ---------------------------------------------------------------------
 
 ACT_SHAPES = [([1], 1, 0, 0), ([0, 5, 0], 64, 0, 0), ([127, 2, 128, 300, 0, 1], 264, 8, 8), ([1000], 520, 0, 0), ([40, 260], 1003, 5, 1),
-              ([1] * 700 + [0] * 50, 24, 0, 0), ([128, 128, 0, 128], 2048, 0, 0), ([0, 0], 40, 0, 0), ([3000, 1], 8, 0, 0)]
+              ([1] * 700 + [0] * 50, 24, 0, 0), ([128, 128, 0, 128], 2048, 0, 0), ([0, 0], 40, 0, 0), ([3000, 1], 8, 0, 0),
+              ([33, 7, 64, 0, 31, 32, 200], 1258, 0, 0), ([9000, 1, 400], 300, 2, 2)]
 
 
 @pytest.mark.gpu
