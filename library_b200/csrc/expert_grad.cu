@@ -17,14 +17,14 @@ constexpr int kActThreads = 256;
 constexpr int kActWarps = kActThreads / 32;
 constexpr int kActBatch = 4;  // rows in flight per warp
 
-__device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e, int segments, int rows) {
+__device__ __forceinline__ int clamp_row(const int32_t* off, int e, int segments, int rows) {
   if (!off) return e == 0 ? 0 : rows;
   const int v = off[e];
   return v < 0 ? 0 : v > rows ? rows : v;
 }
 
 // The last segment that begins at or before row r (0 if none does).  Whole warp.
-__device__ __forceinline__ int segment_of(const int32_t* __restrict__ off, int segments, int rows, int r) {
+__device__ __forceinline__ int segment_of(const int32_t* off, int segments, int rows, int r) {
   const int lane = threadIdx.x & 31, per = (segments + 31) / 32;
   const unsigned hi = __ballot_sync(0xffffffffu, lane * per < segments && clamp_row(off, lane * per, segments, rows) <= r);
   if (hi == 0) return 0;
@@ -36,7 +36,7 @@ __device__ __forceinline__ int segment_of(const int32_t* __restrict__ off, int s
 template <typename T, int V, int U, int ACT>
 __global__ void __launch_bounds__(kActThreads, 3)
 expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz, int64_t lddz,
-                       float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
+                       float* __restrict__ dbias, int64_t lddb, const int32_t* off, int segments, int rows,
                        int cols, int strips, int warp_rows, float* __restrict__ pieces) {
   constexpr int kStrip = 32 * V * U;
   __shared__ float head[kActWarps][kStrip], tail[kActWarps][kStrip];
@@ -146,8 +146,8 @@ expert_act_grad_kernel(const T* dy, int64_t lddy, const T* z, int64_t ldz, T* dz
 // 64 columns of one segment's dBias per CTA: quarter q of the CTA adds the pieces of every fourth chunk, then the quarters are joined.
 constexpr int kJoinCols = 64, kJoinParts = kActThreads / kJoinCols;
 __global__ void __launch_bounds__(kActThreads)
-expert_bias_join_kernel(float* __restrict__ dbias, int64_t lddb, const int32_t* __restrict__ off, int segments, int rows,
-                        int cols, int strips, int chunk_rows, const float* __restrict__ pieces) {
+expert_bias_join_kernel(float* __restrict__ dbias, int64_t lddb, const int32_t* off, int segments, int rows,
+                        int cols, int strips, int chunk_rows, const float* pieces) {
   __shared__ float part[kJoinParts][kJoinCols];
   dependency_wait();
   dependents_go();

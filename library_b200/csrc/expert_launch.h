@@ -1,6 +1,8 @@
 // Launches of the expert kernels.  A layer is a chain of short kernels on one stream: each is launched as a programmatic dependent of
 // the one before, so that its blocks are placed, its barriers and tensor memory set up and its tensor maps
 // fetched while the last blocks of that one still run.
+// Inputs are not declared const __restrict__: the compiler may take such memory for constant over the whole kernel and move its
+// loads above the wait.
 // Every kernel here calls dependency_wait() in every thread before it touches global memory (it returns when the kernels before
 // have finished and their results are visible), and dependents_go() once it holds all it needs of its SM - after
 // tensor memory has been allocated: a dependent's block could otherwise take it first and both would wait for good.

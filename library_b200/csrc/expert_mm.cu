@@ -222,7 +222,7 @@ struct MmArgs {
   int* err;
 };
 
-__device__ __forceinline__ int clamp_row(const int32_t* __restrict__ off, int e, int rows) {
+__device__ __forceinline__ int clamp_row(const int32_t* off, int e, int rows) {
   const int v = off[e];
   return v < 0 ? 0 : v > rows ? rows : v;
 }
@@ -909,7 +909,7 @@ struct Copy16 {
 // loads in flight per lane (bound by HBM: 1 GB moved for 27 blocks of 3,224 x 2,965).
 template <typename U>
 __global__ void __launch_bounds__(256)
-expert_repack_kernel(const __grid_constant__ Copy16 a, const __grid_constant__ Copy16 b, const int32_t* __restrict__ off, int rows) {
+expert_repack_kernel(const __grid_constant__ Copy16 a, const __grid_constant__ Copy16 b, const int32_t* off, int rows) {
   dependency_wait();
   dependents_go();
   const int lane = threadIdx.x & 31;
@@ -1149,6 +1149,7 @@ alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t h, alphasparseOperat
   if (z && (s = expert_check_mat(z, shape.rows, shape.n)) != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   if (shape.rows == 0 || shape.n == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
   if (!buffer && repack_bytes(x, w)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  if (!impl(h)->dev_err) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;  // a handle that alphasparseGetHandle has not set up
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
   const bool nk = op == ALPHA_SPARSE_OPERATION_TRANSPOSE;
@@ -1211,6 +1212,7 @@ alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t h, alphasparse
   alphasparseDnMatDescr_t m = nk ? x : dz, j = nk ? dz : x;  // columns and rows of a block of dW
   if (m->cols == 0 || j->cols == 0) return ALPHA_SPARSE_STATUS_SUCCESS;
   if (!buffer && repack_bytes(x, dz)) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  if (!impl(h)->dev_err) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;  // a handle that alphasparseGetHandle has not set up
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
   Operand om, oj;

@@ -44,7 +44,7 @@ __device__ __forceinline__ SlotRange warp_slots(int64_t slots) {
   return {begin, begin + per < slots ? begin + per : slots};
 }
 template <typename Id>
-__device__ __forceinline__ void load_ids(const Id* __restrict__ ids, int64_t s, int64_t end, int experts, int (&id)[kSortBatch]) {
+__device__ __forceinline__ void load_ids(const Id* ids, int64_t s, int64_t end, int experts, int (&id)[kSortBatch]) {
 #pragma unroll
   for (int i = 0; i < kSortBatch; ++i) {
     id[i] = -1;
@@ -57,7 +57,7 @@ __device__ __forceinline__ void load_ids(const Id* __restrict__ ids, int64_t s, 
 
 // counts[e][w]: the slots of e that the CTA's warps before w hold.  totals[e]: the CTA's.
 template <typename Id>
-__device__ __forceinline__ void count_slots(const Id* __restrict__ ids, int experts, SlotRange r, int* counts, int* totals) {
+__device__ __forceinline__ void count_slots(const Id* ids, int experts, SlotRange r, int* counts, int* totals) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int id[kSortBatch];
   load_ids(ids, r.begin + lane, r.end, experts, id);  // on their way while the counts are cleared
@@ -92,7 +92,7 @@ __device__ __forceinline__ void count_slots(const Id* __restrict__ ids, int expe
 
 // position[] of the warp's slots: base[e] is where the CTA's first slot of e goes.
 template <typename Id, int BITS>
-__device__ __forceinline__ void place_slots(const Id* __restrict__ ids, int experts, SlotRange r, int* counts, const int* base,
+__device__ __forceinline__ void place_slots(const Id* ids, int experts, SlotRange r, int* counts, const int* base,
                                             int32_t* __restrict__ position) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t s = r.begin + lane; s - lane < r.end; s += 32 * kSortBatch) {
@@ -157,7 +157,7 @@ __device__ int scan_experts(int* all, int experts, int* warp_sums) {
 // The whole sort in one launch of one thread-block cluster: counts meet in distributed shared memory.
 template <typename Id, int BITS>
 __global__ void __launch_bounds__(kSortThreads)
-route_sort_cluster_kernel(const Id* __restrict__ ids, int64_t slots, int experts, int32_t* __restrict__ offsets,
+route_sort_cluster_kernel(const Id* ids, int64_t slots, int experts, int32_t* __restrict__ offsets,
                           int32_t* __restrict__ position) {
   extern __shared__ int sort_smem[];
   int* counts = sort_smem;
@@ -204,7 +204,7 @@ route_sort_cluster_kernel(const Id* __restrict__ ids, int64_t slots, int experts
 // those of the CTAs before it and all of them, and places its slots.
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
-route_sort_count_kernel(const Id* __restrict__ ids, int64_t slots, int experts, int* __restrict__ before) {
+route_sort_count_kernel(const Id* ids, int64_t slots, int experts, int* __restrict__ before) {
   extern __shared__ int sort_smem[];
   int* totals = sort_smem + experts * kSortRow;
   dependency_wait();
@@ -214,7 +214,7 @@ route_sort_count_kernel(const Id* __restrict__ ids, int64_t slots, int experts, 
 }
 template <typename Id, int BITS>
 __global__ void __launch_bounds__(kSortThreads)
-route_sort_place_kernel(const Id* __restrict__ ids, int64_t slots, int experts, const int* __restrict__ before,
+route_sort_place_kernel(const Id* ids, int64_t slots, int experts, const int* before,
                         int32_t* __restrict__ offsets, int32_t* __restrict__ position) {
   extern __shared__ int sort_smem[];
   int* counts = sort_smem;
@@ -257,8 +257,8 @@ constexpr int kRowThreads = 256;
 // A warp takes a token's stretch of 32 * U packs: loads it once, stores it to every sorted row.
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
-route_dispatch_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs, int64_t ldxs,
-                      const int32_t* __restrict__ position, int tokens, int topk, int packs, int stretches, int xs_rows) {
+route_dispatch_kernel(const T* x, int64_t ldx, T* __restrict__ xs, int64_t ldxs,
+                      const int32_t* position, int tokens, int topk, int packs, int stretches, int xs_rows) {
   const int lane = threadIdx.x & 31;
   const int64_t task = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
   dependency_wait();
@@ -289,8 +289,8 @@ route_dispatch_kernel(const T* __restrict__ x, int64_t ldx, T* __restrict__ xs, 
 // warps that walk over several stretches 90 us (neighbouring stretches of a row then run at different times).
 template <typename T, int V, int U, int J>
 __global__ void __launch_bounds__(kRowThreads, 3)
-route_combine_kernel(const T* __restrict__ ys, int64_t ldys, const float* __restrict__ weights, const T* r, int64_t ldr,
-                     T* y, int64_t ldy, const int32_t* __restrict__ position, int tokens, int topk, int packs,
+route_combine_kernel(const T* ys, int64_t ldys, const float* weights, const T* r, int64_t ldr,
+                     T* y, int64_t ldy, const int32_t* position, int tokens, int topk, int packs,
                      int stretches, int ys_rows) {
   const int lane = threadIdx.x & 31;
   const int64_t task = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
@@ -380,9 +380,9 @@ __device__ __forceinline__ float reduce_values(float (&v)[J], int lane) {
 constexpr int kGradThreads = 128;  // of a token
 template <typename T, int V, int U, int J>
 __global__ void __launch_bounds__(kRowThreads, 4)
-route_combine_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* ys, int64_t ldys,
-                          const float* __restrict__ weights, T* dys, int64_t lddys, float* __restrict__ dweights,
-                          const int32_t* __restrict__ position, int tokens, int topk, int packs, int rows) {
+route_combine_grad_kernel(const T* dy, int64_t lddy, const T* ys, int64_t ldys,
+                          const float* weights, T* dys, int64_t lddys, float* __restrict__ dweights,
+                          const int32_t* position, int tokens, int topk, int packs, int rows) {
   __shared__ float part[kRowThreads / 32][J];
   const int t = (int)blockIdx.x * (int)blockDim.y + (int)threadIdx.y;
   dependency_wait();

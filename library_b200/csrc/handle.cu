@@ -129,6 +129,7 @@ alphasparseStatus_t alphasparseGetStream(alphasparseHandle_t h, cudaStream_t* st
 alphasparseStatus_t alphasparseGetDeviceError(alphasparseHandle_t h, int* flag) {
   if (!h) return ALPHA_SPARSE_STATUS_INVALID_HANDLE;
   if (!flag) return ALPHA_SPARSE_STATUS_INVALID_POINTER;
+  if (!impl(h)->dev_err) return ALPHA_SPARSE_STATUS_NOT_INITIALIZED;
   DeviceScope dev(h->device);
   ASP_CUDA(dev.status);
   ASP_CUDA(cudaMemcpyAsync(flag, impl(h)->dev_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream));
