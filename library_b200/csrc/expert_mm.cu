@@ -672,44 +672,43 @@ __device__ __forceinline__ bool few_tile(int j, const MmArgs& a, Tile& x) {
 
 __device__ __forceinline__ float ld_peer(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
 }
+
+constexpr int kFewSplit = 8;  // CTAs that may share a tile's contraction (the portable cluster size)
 
 template <typename TO, int ACT>
 __device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, int64_t row0, int m, int col, uint32_t sums, uint32_t rank,
                                               uint32_t size, bool in, float bias) {
-  // four rows at a time, their partial sums of all CTAs in flight together
-  for (int j0 = (int)rank; j0 < x.rows; j0 += (int)size * 4) {
-    float v[4];
+  if (!in) return;
+  // two rows at a time, the sums of all CTAs asked for before the first is added
+  for (int j0 = (int)rank; j0 < x.rows; j0 += (int)size * 2) {
+    const int j1 = j0 + (int)size;
+    const bool second = j1 < x.rows;
+    float p[2][kFewSplit];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = 0.f;
-    TO res[4];
-    if (!in) continue;
-    if (a.r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + i * (int)size;
-        if (j < x.rows) res[i] = ((const TO*)a.r)[(row0 + j) * a.ldr + m];
-      }
-    }
-    for (uint32_t c = 0; c < size; ++c) {
-      const uint32_t from = peer_u32(sums, c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + i * (int)size;
-        if (j < x.rows) v[i] += ld_peer(from + (uint32_t)(j * kTileM + col) * 4u);
+    for (int c = 0; c < kFewSplit; ++c) {
+      if ((uint32_t)c < size) {
+        const uint32_t from = peer_u32(sums, c) + (uint32_t)col * 4u;
+        p[0][c] = ld_peer(from + (uint32_t)(j0 * kTileM) * 4u);
+        if (second) p[1][c] = ld_peer(from + (uint32_t)(j1 * kTileM) * 4u);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = j0 + i * (int)size;
-      if (j >= x.rows) continue;
-      const int64_t row = row0 + j;
-      float w = v[i] + bias;
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && !second) break;
+      const int64_t row = row0 + (i == 0 ? j0 : j1);
+      TO res;
+      if (a.r) res = ((const TO*)a.r)[row * a.ldr + m];
+      float w = 0.f;
+#pragma unroll
+      for (int c = 0; c < kFewSplit; ++c)
+        if ((uint32_t)c < size) w += p[i][c];
+      w += bias;
       if (a.z) ((TO*)a.z)[row * a.ldz + m] = Wide<TO>::down(w);
       w = activate<ACT>(w);
-      if (a.r) w += Wide<TO>::up(res[i]);
+      if (a.r) w += Wide<TO>::up(res);
       ((TO*)a.y)[row * a.ldy + m] = Wide<TO>::down(w);
     }
   }
@@ -1049,7 +1048,7 @@ alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, con
   // CTAs that share a tile's contraction: as many as fit the device at once, a ring's worth of stages each
   const int resident = (J == 16 ? 3 : 2) * impl(h)->sm_count;
   int size = 1;
-  while (size < 8 && tiles * size * 2 <= resident && chunks >= 2 * size * kFewStages) size *= 2;
+  while (size < kFewSplit && tiles * size * 2 <= resident && chunks >= 2 * size * kFewStages) size *= 2;
   return launch_chained(h, kernel, dim3((unsigned)(tiles * size)), dim3(kFewThreads), Few<J>::kSmem, size, ma, mb, a, size);
 }
 template <int KIND, int J>
