@@ -40,6 +40,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -55,7 +57,7 @@ __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The arrival that hands an accumulator back: its reads have completed (tcgen05.wait::ld), nothing else has to be visible.  A release
+// An arrival that only says that reads have completed (of an accumulator, after tcgen05.wait::ld; of a peer's sums).  A release
 // at cluster scope would wait for the epilogue's global stores.
 __device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -68,6 +70,21 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(2000)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+// The same for what a peer's threads wrote before they arrived with a release at cluster scope.
+__device__ __forceinline__ bool mbar_wait_peers(uint32_t bar, uint32_t parity, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity), "r"(2000)
@@ -607,24 +624,35 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 // (and, for gradients, few tiles: a long contraction would run on few SMs).
 // One output tile of 128 columns x up to J rows per CLUSTER, whose CTAs share the contraction: each streams its
 // part of K through a ring of its own (several CTAs per SM, so that many loads are in flight),
-// leaves its fp32 sums in shared memory, and after a cluster barrier CTA r adds up the rows r, r + size, ... over all
+// leaves its fp32 sums in shared memory and tells its peers, and CTA r adds up the rows r, r + size, ... over all
 // CTAs in rank order (through distributed shared memory) and finishes them.  No workspace, no atomics.
 constexpr int kFewThreads = 192;
 constexpr int kFewStages = 4;
 constexpr int kFewBox = 16;                                  // rows of X per TMA box
 template <int J> struct Few {
   static constexpr int kStage = kABytes + J * kKC * 2;
-  static constexpr int kSmem = 1024 + kFewStages * kStage + 8 * (2 * kFewStages + 1) + 8;
+  static constexpr int kSmem = 1024 + kFewStages * kStage + 8 * (2 * kFewStages + 3) + 8;
   static_assert(kFewStages * kStage >= J * kTileM * 4, "the sums take the ring's place");
 };
 constexpr int kFewTmem = 64;
+// Polls of the waits for the cluster's CTAs: two seconds, whatever the limit of the others, since a CTA that gave up still arrives and
+// none may leave while a peer can reach its shared memory.
+constexpr uint32_t kPeerPolls = 1u << 20;
 
 // Row tile j (of at most J rows) over all segments: false if there are fewer tiles.  Whole warp, without shared memory: a lane counts
 // the tiles of consecutive segments, the lanes' sums are scanned, and the lane that holds tile j finds its segment.
 template <int J>
 __device__ __forceinline__ bool few_tile(int j, const MmArgs& a, Tile& x) {
   const int lane = threadIdx.x & 31;
-  auto at = [&](int e) { return a.off ? clamp_row(a.off, e, a.rows) : (e == 0 ? 0 : a.rows); };
+  if (!a.off) {
+    x.e = 0;
+    x.row0 = j * J;
+    if (x.row0 >= a.rows) return false;
+    x.rows = a.rows - x.row0 < J ? a.rows - x.row0 : J;
+    x.width = (x.rows + 15) & ~15;
+    return true;
+  }
+  auto at = [&](int e) { return clamp_row(a.off, e, a.rows); };
   const int per = (a.segments + 31) / 32, e0 = lane * per < a.segments ? lane * per : a.segments;
   const int e1 = e0 + per < a.segments ? e0 + per : a.segments;
   int sum = 0, prev = at(e0);
@@ -717,25 +745,29 @@ __device__ __forceinline__ void finish_shared(const MmArgs& a, const Tile& x, in
 template <int KIND, int J, typename TO>
 __global__ void __launch_bounds__(kFewThreads)
 expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ MmArgs a,
-                     int size) {
+                     int log_size) {
   constexpr int kStage = Few<J>::kStage;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gen = smem_raw + (base - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(gen + kFewStages * kStage);
-  const uint32_t full = base + kFewStages * kStage, empty = full + 8 * kFewStages, acc_full = empty + 8 * kFewStages;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kFewStages + 1);
+  const uint32_t full = base + kFewStages * kStage, empty = full + 8 * kFewStages, acc_full = empty + 8 * kFewStages, ready = acc_full + 8,
+                 done = ready + 8;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kFewStages + 3);
   int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t limit = a.limit & ~kWaitDropCopy;
-  const uint32_t rank = size > 1 ? cluster_rank() : 0u;
-  const int mblocks = (a.m_total + kTileM - 1) / kTileM, t = (int)blockIdx.x / size;
+  const int size = 1 << log_size;
+  const uint32_t rank = blockIdx.x & (uint32_t)(size - 1);  // in the cluster
+  const int mblocks = (a.m_total + kTileM - 1) / kTileM, t = (int)(blockIdx.x >> log_size);
   if (tid == 0) {
     for (int i = 0; i < kFewStages; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(ready, size);
+    mbar_init(done, size);
     *s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -748,6 +780,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *s_tmem;
+  cluster_arrive();  // this CTA's barriers are ready; waited for when the contraction is done, so at no cost
   dependents_go();  // tensor memory is allocated
   dependency_wait();
   Tile x;
@@ -764,6 +797,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   } else {
     if (!few_tile<J>(t / mblocks, a, x)) {  // the whole cluster: the grid covers the most tiles these sizes can have
       if (warp == 1) tmem_free<1>(tmem, kFewTmem);
+      cluster_wait();
       return;
     }
     x.k0 = 0;
@@ -772,7 +806,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   }
   x.m0 = (t % mblocks) * kTileM;
   const int chunks = x.klen > 0 ? (x.klen + kKC - 1) / kKC : 0;
-  const int c0 = (int)((int64_t)chunks * rank / size), c1 = (int)((int64_t)chunks * (rank + 1) / size);
+  const int c0 = (int)(((uint32_t)chunks * rank) >> log_size), c1 = (int)(((uint32_t)chunks * (rank + 1)) >> log_size);
   bool ok = true;
   if (warp == 0) {
     const int boxes = KIND == kGradW ? 0 : x.width / kFewBox;
@@ -881,7 +915,16 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (tid == 0) *a.err = 1;
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   }
-  if (size > 1) cluster_sync();  // the peers' sums are complete
+  cluster_wait();
+  if (size > 1) {
+    // this CTA's sums are complete: every peer is told, and waits for all of them (a barrier instruction of the cluster takes a
+    // microsecond, arrivals on each other's barriers half of that)
+    if (tid < size) mbar_arrive(peer_u32(ready, tid));
+    if (epilogue && !__all_sync(0xffffffffu, mbar_wait_peers(ready, 0u, kPeerPolls))) {
+      *s_fail = 1;
+      if (tid == 64) *a.err = 1;
+    }
+  }
   if (epilogue && size > 1 && !*s_fail) {
     switch (KIND == kGradW ? (int)ALPHASPARSE_ACT_NONE : a.act) {
       case ALPHASPARSE_ACT_RELU: finish_shared<TO, ALPHASPARSE_ACT_RELU>(a, x, out_row0, m, col, base, rank, (uint32_t)size, in, bias); break;
@@ -893,7 +936,12 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   __syncwarp();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (warp == 1) tmem_free<1>(tmem, kFewTmem);
-  if (size > 1) cluster_sync();  // no CTA leaves while a peer reads its sums
+  if (size > 1) {
+    // no CTA leaves while a peer reads its sums (what was read has been used: nothing has to be made visible)
+    __syncthreads();
+    if (tid < size) mbar_arrive_relaxed(peer_u32(done, tid));
+    if (warp == 0 && !__all_sync(0xffffffffu, mbar_wait(done, 0u, kPeerPolls)) && lane == 0) *a.err = 1;
+  }
 }
 
 // ---- operands the TMA cannot take: aligned copies -----------------------------------------------
@@ -1047,9 +1095,9 @@ alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, con
   if (s != ALPHA_SPARSE_STATUS_SUCCESS) return s;
   // CTAs that share a tile's contraction: as many as fit the device at once, a ring's worth of stages each
   const int resident = (J == 16 ? 3 : 2) * impl(h)->sm_count;
-  int size = 1;
-  while (size < kFewSplit && tiles * size * 2 <= resident && chunks >= 2 * size * kFewStages) size *= 2;
-  return launch_chained(h, kernel, dim3((unsigned)(tiles * size)), dim3(kFewThreads), Few<J>::kSmem, size, ma, mb, a, size);
+  int log_size = 0;
+  while ((1 << log_size) < kFewSplit && (tiles << log_size) * 2 <= resident && chunks >= ((2 * kFewStages) << log_size)) ++log_size;
+  return launch_chained(h, kernel, dim3((unsigned)(tiles << log_size)), dim3(kFewThreads), Few<J>::kSmem, 1 << log_size, ma, mb, a, log_size);
 }
 template <int KIND, int J>
 alphasparseStatus_t launch_few(alphasparseHandle_t h, const CUtensorMap& ma, const CUtensorMap& mb, const MmArgs& a, int64_t tiles,
