@@ -432,7 +432,8 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     prefetch_map(&map_b);
   }
   __syncthreads();
-  dependents_go();  // tensor memory is allocated
+  cluster_arrive();  // this CTA's barriers are ready (the wait is below, behind the kernel's other waits)
+  dependents_go();   // tensor memory is allocated
   dependency_wait();
   for (int i = tid; i <= a.segments; i += kMmThreads) s_off[i] = a.off ? clamp_row(a.off, i, a.rows) : (i == 0 ? 0 : a.rows);
   __syncthreads();
@@ -445,7 +446,7 @@ expert_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  cluster_sync();  // the peer's barriers are ready
+  cluster_wait();  // the peer's barriers are ready
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *s_tmem;
   const int first = (int)blockIdx.x / 2, stride = (int)gridDim.x / 2;
