@@ -455,6 +455,15 @@ def _ptr(t: torch.Tensor | None):
     return t.data_ptr() if t is not None else None
 
 
+def _workspace(buffer: torch.Tensor | None, needed):
+    """Pointer of a workspace that holds needed() bytes.  (The C calls cannot see a buffer's size, and the bytes depend on
+    the operands' alignment: a buffer sized for other operands would be written past its end.)"""
+    if buffer is None:
+        return None
+    assert buffer.is_cuda and buffer.is_contiguous() and buffer.numel() * buffer.element_size() >= needed()
+    return buffer.data_ptr()
+
+
 def _gates(routing: Routing, w: torch.Tensor | None):
     """Pointer of a tokens x topk fp32 array (or NULL)."""
     assert w is None or (w.is_cuda and w.dtype == torch.float32 and w.is_contiguous() and w.numel() == routing.tokens * routing.topk)
@@ -477,7 +486,8 @@ def routing_buffer_size(handle: Handle, routing: Routing) -> int:
 
 def routing_sort(handle: Handle, routing: Routing, buffer: torch.Tensor | None = None):
     """Fill routing.offsets and routing.position from routing.expert_ids (asynchronous, like every call below)."""
-    _check(load().alphasparseRoutingSort(handle.h, routing.d, _ptr(buffer)), "alphasparseRoutingSort")
+    _check(load().alphasparseRoutingSort(handle.h, routing.d, _workspace(buffer, lambda: routing_buffer_size(handle, routing))),
+           "alphasparseRoutingSort")
 
 
 def routing_dispatch(handle: Handle, routing: Routing, X: DnMat, Xs: DnMat):
@@ -514,7 +524,8 @@ def expert_mm(handle: Handle, X: DnMat, W: DnMat, Y: DnMat, offsets: torch.Tenso
     op OP_T: W stacks N x K blocks; OP_N: K x N blocks.  ``buffer``: expert_mm_buffer_size bytes (none when that is 0)."""
     n, off = _segments(offsets)
     _check(load().alphasparseExpertMM(handle.h, op, n, off, X.d, W.d, _d(bias), act, _d(residual), _d(preact), Y.d,
-                                      _ptr(buffer)), "alphasparseExpertMM")
+                                      _workspace(buffer, lambda: expert_mm_buffer_size(handle, X, W, Y, offsets, op))),
+           "alphasparseExpertMM")
 
 
 def expert_mm_grad_weight_buffer_size(handle: Handle, X: DnMat, dZ: DnMat, dW: DnMat, offsets: torch.Tensor | None = None,
@@ -530,7 +541,8 @@ def expert_mm_grad_weight(handle: Handle, X: DnMat, dZ: DnMat, dW: DnMat, offset
                           buffer: torch.Tensor | None = None):
     """dW_e = dZ_e^T X_e (OP_T) or X_e^T dZ_e (OP_N), stacked like W."""
     n, off = _segments(offsets)
-    _check(load().alphasparseExpertMM_gradW(handle.h, op, n, off, X.d, dZ.d, dW.d, _ptr(buffer)),
+    _check(load().alphasparseExpertMM_gradW(handle.h, op, n, off, X.d, dZ.d, dW.d,
+                                            _workspace(buffer, lambda: expert_mm_grad_weight_buffer_size(handle, X, dZ, dW, offsets, op))),
            "alphasparseExpertMM_gradW")
 
 
@@ -547,7 +559,8 @@ def expert_act_grad(handle: Handle, dY: DnMat, Z: DnMat | None, dZ: DnMat | None
                     act=ACT_NONE, dbias: DnMat | None = None, buffer: torch.Tensor | None = None):
     """dZ = dY * act'(Z) and dbias[e] = column sums of dZ over segment e.  ``buffer``: needed with dbias."""
     n, off = _segments(offsets)
-    _check(load().alphasparseExpertActGrad(handle.h, n, off, act, dY.d, _d(Z), _d(dZ), _d(dbias), _ptr(buffer)),
+    _check(load().alphasparseExpertActGrad(handle.h, n, off, act, dY.d, _d(Z), _d(dZ), _d(dbias),
+                                           _workspace(buffer, lambda: expert_act_grad_buffer_size(handle, dY, offsets, act, dbias))),
            "alphasparseExpertActGrad")
 
 

@@ -764,6 +764,49 @@ def test_product_gradients_against_differences(h):
 
 
 @pytest.mark.gpu
+def test_combine_gradient_against_differences(h):
+    """L = sum(dY * combine(Ys, w)) is linear in Ys and in w: a directional difference is exact up to rounding."""
+    tokens, topk, width = 40, 3, 88
+    r = routed(tokens, topk, 6, 4)
+    g = gen(8)
+    ys, dy = torch.randn(tokens * topk, width, device="cuda", generator=g), torch.randn(tokens, width, device="cuda", generator=g)
+    w = torch.randn(tokens, topk, device="cuda", generator=g)
+    dys, dw = torch.zeros_like(ys), torch.zeros_like(w)
+    api.routing_combine_grad(h, r, api.DnMat(dy), api.DnMat(ys), api.DnMat(dys), w, dw)
+    pos, kept = r.position.long(), (r.position >= 0).double()
+
+    def loss(ys, w):
+        rows = ys[pos.clamp(min=0)] * (w * kept)[:, :, None]
+        return (dy.double() * rows.sum(1)).sum()
+
+    vy, vw = torch.randn_like(ys).double(), torch.randn_like(w).double()
+    for got, v, diff in ((dys, vy, loss(ys.double() + vy, w.double()) - loss(ys.double() - vy, w.double())),
+                         (dw, vw, loss(ys.double(), w.double() + vw) - loss(ys.double(), w.double() - vw))):
+        # dys: one rounding an element; dw: fp32 sums of 88 products whose sizes add up to less than 16 times their sum in the mean
+        assert abs(float(diff / 2 - (got.double() * v).sum())) <= float(96 * 2 * U * 16 * (got.double() * v).abs().sum())
+
+
+@pytest.mark.gpu
+def test_a_workspace_that_is_too_small_is_refused(h):
+    x, w = torch.zeros(9, 33, device="cuda", dtype=torch.float16), torch.zeros(20, 33, device="cuda", dtype=torch.float16)
+    y, dw = torch.zeros(9, 20, device="cuda", dtype=torch.float16), torch.zeros(20, 33, device="cuda", dtype=torch.float16)
+    X, W, Y, D = api.DnMat(x), api.DnMat(w), api.DnMat(y), api.DnMat(dw)
+    small = torch.zeros(16, dtype=torch.uint8, device="cuda")
+    for call in (lambda b: api.expert_mm(h, X, W, Y, buffer=b), lambda b: api.expert_mm_grad_weight(h, X, Y, D, buffer=b)):
+        with pytest.raises(AssertionError):
+            call(small)
+        with pytest.raises(api.AlphaSparseError) as e:
+            call(None)
+        assert e.value.status == 7
+    db = torch.zeros(1, 20, device="cuda")
+    with pytest.raises(AssertionError):
+        api.expert_act_grad(h, Y, None, None, None, api.ACT_NONE, api.DnMat(db), small)
+    r = api.Routing(torch.zeros(20000, 2, dtype=torch.int32, device="cuda"), 6)
+    with pytest.raises(AssertionError):
+        api.routing_sort(h, r, small)
+
+
+@pytest.mark.gpu
 def test_captured_layer_and_other_streams(h):
     """The whole layer captured into a graph and replayed on new inputs, and run on a stream of its own, gives the bits of the
     plain call; a second layer with its own workspace runs beside it."""
