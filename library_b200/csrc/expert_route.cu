@@ -356,7 +356,7 @@ route_combine_kernel(const T* ys, int64_t ldys, const float* weights, const T* r
 
 // Sums of J values over the lanes of a warp (J a power of two, at most 32): lane l ends with the sum of value l % J.
 // While more than one value is left, each step sends half of them to the partner and adds the half that comes back:
-// 9 shuffles for J = 8 instead of 40.
+// 5 shuffles for J = 2 instead of 10.
 template <int J>
 __device__ __forceinline__ float reduce_values(float (&v)[J], int lane) {
 #pragma unroll
@@ -375,9 +375,8 @@ __device__ __forceinline__ float reduce_values(float (&v)[J], int lane) {
 
 // Gradient of combine.  blockDim.y tokens per CTA, blockDim.x threads on a token's row (whole warps).  J slots at a time: their rows
 // of Ys are all asked for before the first is used; their dot products are added up over lanes, then over the row's warps, in a
-// fixed order.  Bound by HBM (435 MB at 8,192 tokens x 6 rows of 2,048 bf16: 68 us at 6.4 TB/s): four rows in flight, two tokens per CTA
-// and four CTAs per SM take 81 us; one token per CTA 90 us; eight rows in flight (three CTAs fit) 105 us, without a register limit
-// (one CTA) 189 us.
+// fixed order.  Bound by HBM (435 MB at 8,192 tokens x 6 rows of 2,048 bf16: 68 us at 6.4 TB/s): 1 KB of two rows per warp in flight,
+// two tokens per CTA and four CTAs per SM take 71.7 us; 512 bytes of four rows 82 us (one token per CTA 90), of eight rows 105 us.
 constexpr int kGradThreads = 128;  // of a token
 template <typename T, int V, int U, int J>
 __global__ void __launch_bounds__(kRowThreads, 4)
@@ -390,13 +389,15 @@ route_combine_grad_kernel(const T* dy, int64_t lddy, const T* ys, int64_t ldys,
   dependents_go();
   const int lane = threadIdx.x & 31;
   const int warps = (int)blockDim.x >> 5, row_warp0 = (int)threadIdx.y * warps, my_warp = row_warp0 + ((int)threadIdx.x >> 5);
+  int p_mine = -1;
+  float w_mine = 1.f;
   for (int j0 = 0; j0 < topk; j0 += J) {
-    // lane i of every warp holds slot j0 + i
-    int p_mine = -1;
-    float w_mine = 1.f;
-    if (t < tokens && lane < J && j0 + lane < topk) {
-      p_mine = position[(int64_t)t * topk + j0 + lane];
-      if (weights) w_mine = weights[(int64_t)t * topk + j0 + lane];
+    if ((j0 & 31) == 0) {  // lane i of every warp holds slot i of the next 32
+      p_mine = -1;
+      if (t < tokens && j0 + lane < topk) {
+        p_mine = position[(int64_t)t * topk + j0 + lane];
+        if (weights) w_mine = weights[(int64_t)t * topk + j0 + lane];
+      }
     }
     float dot[J];
 #pragma unroll
@@ -413,7 +414,7 @@ route_combine_grad_kernel(const T* dy, int64_t lddy, const T* ys, int64_t ldys,
         if (dweights) {
 #pragma unroll
           for (int i = 0; i < J; ++i) {
-            const int p = __shfl_sync(0xffffffffu, p_mine, i);
+            const int p = __shfl_sync(0xffffffffu, p_mine, (j0 + i) & 31);
             if ((unsigned)p >= (unsigned)rows) continue;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -424,8 +425,8 @@ route_combine_grad_kernel(const T* dy, int64_t lddy, const T* ys, int64_t ldys,
         }
 #pragma unroll
         for (int i = 0; i < J; ++i) {
-          const int p = __shfl_sync(0xffffffffu, p_mine, i);
-          const float w = __shfl_sync(0xffffffffu, w_mine, i);
+          const int p = __shfl_sync(0xffffffffu, p_mine, (j0 + i) & 31);
+          const float w = __shfl_sync(0xffffffffu, w_mine, (j0 + i) & 31);
           if ((unsigned)p >= (unsigned)rows) continue;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -453,7 +454,7 @@ route_combine_grad_kernel(const T* dy, int64_t lddy, const T* ys, int64_t ldys,
       for (int k = 0; k < warps; ++k) sum += part[row_warp0 + k][threadIdx.x];
       dweights[(int64_t)t * topk + j0 + threadIdx.x] = sum;
     }
-    __syncthreads();
+    if (j0 + J < topk) __syncthreads();  // part is written again
   }
 }
 
@@ -541,11 +542,11 @@ alphasparseStatus_t run_combine_grad(alphasparseHandle_t h, alphasparseRoutingDe
                                      float* dweights, int64_t rows) {
   const int64_t packs = dy->cols / V;
   int x = 32;
-  constexpr int U = packs_per_lane<T, V>(16);
+  constexpr int U = packs_per_lane<T, V>(32);
   while (x < kGradThreads && (int64_t)x * U < packs) x *= 2;
   const int y = kRowThreads / x;
   const int64_t blocks = (r->tokens + y - 1) / y;
-  return launch_chained(h, route_combine_grad_kernel<T, V, U, 4>, dim3((unsigned)blocks), dim3(x, y), 0, 1,
+  return launch_chained(h, route_combine_grad_kernel<T, V, U, 2>, dim3((unsigned)blocks), dim3(x, y), 0, 1,
       (const T*)dy->values, dy->ld, ys ? (const T*)ys->values : nullptr, ys ? ys->ld : 0, weights,
       dys ? (T*)dys->values : nullptr, dys ? dys->ld : 0, dweights, r->position, (int)r->tokens, (int)r->topk, (int)packs,
       (int)rows);
