@@ -526,6 +526,33 @@ def test_non_finite_values_stay_in_their_rows(h):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("op", [api.OP_T, api.OP_N])
+@pytest.mark.parametrize("rows,n,k", [(5, 200, 64), (16, 64, 200), (41, 392, 64), (2305, 1288, 64), (7, 136, 2048), (35, 72, 1100)])
+def test_a_row_has_the_same_bits_whatever_its_neighbours_hold(h, rows, n, k, op, act):
+    """Rows are independent: with every odd row and every row behind the last segment replaced (by other numbers, infinities, NaN),
+    the even rows of Y and Z keep their bits, in fp32 so that a difference in the last place shows.  The sizes run the kernel
+    for few rows with tiles of 16 and 64, alone and with a shared contraction, and the pair kernel."""
+    g = gen(rows + n)
+    x = torch.randn(rows + 9, k, device="cuda", generator=g).to(torch.bfloat16)
+    w = (torch.randn(n, k, device="cuda", generator=g) * k ** -0.5).to(torch.bfloat16)
+    w = w if op == api.OP_T else w.t().contiguous()
+    off = offsets_of([rows])
+    first = None
+    for scale in (1.0, 0.5, 40.0, float("inf"), float("nan")):
+        x2 = x.clone()
+        x2[1::2] *= scale
+        x2[rows:] *= scale
+        y, z = torch.zeros(rows + 9, n, device="cuda"), torch.zeros(rows + 9, n, device="cuda")
+        X, W, Y = api.DnMat(x2), api.DnMat(w), api.DnMat(y)
+        api.expert_mm(h, X, W, Y, off, op, None, act, None, api.DnMat(z), buffer(api.expert_mm_buffer_size(h, X, W, Y, off, op)))
+        got = [t[:rows:2].clone().view(torch.int32) for t in (y, z)]
+        first = got if first is None else first
+        assert torch.equal(got[1], first[1])
+        assert torch.equal(got[0], first[0]), int((got[0] != first[0]).sum())
+
+
+@pytest.mark.gpu
 def test_offsets_outside_the_rows(h):
     """Offsets are clamped to the rows; descending ones give an empty segment."""
     off = torch.tensor([-5, 3, 2, 900], dtype=torch.int32, device="cuda")
