@@ -41,6 +41,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// (for threads whose reads of a peer's memory have been used and that have nothing to make visible: no wait for their stores)
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -57,8 +59,8 @@ __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// An arrival that only says that reads have completed (of an accumulator, after tcgen05.wait::ld; of a peer's sums).  A release
-// at cluster scope would wait for the epilogue's global stores.
+// An arrival that only says that reads of an accumulator have completed (after tcgen05.wait::ld).  A release at cluster scope would
+// wait for the epilogue's global stores.
 __device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -632,12 +634,13 @@ constexpr int kFewStages = 4;
 constexpr int kFewBox = 16;                                  // rows of X per TMA box
 template <int J> struct Few {
   static constexpr int kStage = kABytes + J * kKC * 2;
-  static constexpr int kSmem = 1024 + kFewStages * kStage + 8 * (2 * kFewStages + 3) + 8;
+  static constexpr int kSmem = 1024 + kFewStages * kStage + 8 * (2 * kFewStages + 2) + 8;
   static_assert(kFewStages * kStage >= J * kTileM * 4, "the sums take the ring's place");
 };
 constexpr int kFewTmem = 64;
-// Polls of the waits for the cluster's CTAs: two seconds, whatever the limit of the others, since a CTA that gave up still arrives and
-// none may leave while a peer can reach its shared memory.
+// The wait for the cluster's sums takes twice the limit of the other waits and this many polls more: a CTA that gives up after its own
+// limit still arrives, so its peers do not give up before it.  (Memory does not depend on it: no CTA leaves before the
+// cluster's last barrier, which every CTA reaches, since every wait before it ends.)
 constexpr uint32_t kPeerPolls = 1u << 20;
 
 // Row tile j (of at most J rows) over all segments: false if there are fewer tiles.  Whole warp, without shared memory: a lane counts
@@ -752,9 +755,8 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* gen = smem_raw + (base - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(gen + kFewStages * kStage);
-  const uint32_t full = base + kFewStages * kStage, empty = full + 8 * kFewStages, acc_full = empty + 8 * kFewStages, ready = acc_full + 8,
-                 done = ready + 8;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kFewStages + 3);
+  const uint32_t full = base + kFewStages * kStage, empty = full + 8 * kFewStages, acc_full = empty + 8 * kFewStages, ready = acc_full + 8;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kFewStages + 2);
   int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t limit = a.limit & ~kWaitDropCopy;
@@ -768,7 +770,6 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
     mbar_init(acc_full, 1);
     mbar_init(ready, size);
-    mbar_init(done, size);
     *s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -822,8 +823,8 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
       if (elect_one()) {
         const uint32_t sa = base + st * kStage, sb = sa + kABytes, bar = full + 8 * st;
         mbar_arrive_tx(bar, bytes);
-        if (a.limit & kWaitDropCopy) {
-          // testing, as in the kernel above
+        if ((a.limit & kWaitDropCopy) && rank == 0) {
+          // testing, as in the kernel above; one CTA of a cluster, so that its peers have to wait for one that gives up
         } else if constexpr (KIND == kFwdT) {
           tma_3d<1>(sa, &map_a, c * kKC, x.m0, x.e, bar);
         } else if constexpr (KIND == kGradW) {
@@ -921,7 +922,7 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     // this CTA's sums are complete: every peer is told, and waits for all of them (a barrier instruction of the cluster takes a
     // microsecond, arrivals on each other's barriers half of that)
     if (tid < size) mbar_arrive(peer_u32(ready, tid));
-    if (epilogue && !__all_sync(0xffffffffu, mbar_wait_peers(ready, 0u, kPeerPolls))) {
+    if (epilogue && !__all_sync(0xffffffffu, mbar_wait_peers(ready, 0u, 2 * limit + kPeerPolls))) {
       *s_fail = 1;
       if (tid == 64) *a.err = 1;
     }
@@ -935,14 +936,15 @@ expert_mm_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
   }
   __syncwarp();
+  if (size > 1) {
+    // the epilogue's warps have read their peers' sums; warp 0's arrivals on the peers' barriers must have landed (a peer that gave up
+    // `ready` has not waited for them)
+    if (warp == 0) cluster_arrive();
+    else cluster_arrive_relaxed();
+  }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (warp == 1) tmem_free<1>(tmem, kFewTmem);
-  if (size > 1) {
-    // no CTA leaves while a peer reads its sums (what was read has been used: nothing has to be made visible)
-    __syncthreads();
-    if (tid < size) mbar_arrive_relaxed(peer_u32(done, tid));
-    if (warp == 0 && !__all_sync(0xffffffffu, mbar_wait(done, 0u, kPeerPolls)) && lane == 0) *a.err = 1;
-  }
+  if (size > 1) cluster_wait();  // no CTA leaves while a peer can reach its shared memory
 }
 
 // ---- operands the TMA cannot take: aligned copies -----------------------------------------------

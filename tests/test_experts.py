@@ -607,6 +607,41 @@ def test_waits_that_run_out_are_reported(monkeypatch):
     assert api.device_error(fresh) == 0
 
 
+# rows, N, K of few-row products whose CTAs share the contraction (from 8 chunks of 64 on, 2 to 8 to a cluster; tiles of 16 and
+# of 64 rows), and of weight gradients that do (more than 512 rows, few tiles)
+SHARED = [("mm", 5, 512, 1024), ("mm", 40, 136, 2048), ("mm", 16, 72, 4104), ("grad", 1100, 64, 96), ("grad", 4133, 200, 72)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,rows,n,k", SHARED)
+def test_a_shared_contraction_whose_wait_runs_out_is_reported(monkeypatch, kind, rows, n, k):
+    """One CTA of every cluster gives up while its peers have their sums: the flag is raised, the peers wait for the one that
+    gave up, and all leave together.  A fresh handle computes the same shapes."""
+    g = gen(rows)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.bfloat16)
+    w = (torch.randn(n, k, device="cuda", generator=g) * k ** -0.5).to(torch.bfloat16)
+    dz = torch.randn(rows, n, device="cuda", generator=g).to(torch.bfloat16)
+    out = torch.zeros((rows, n) if kind == "mm" else (n, k), device="cuda")
+
+    def call(h):
+        if kind == "mm":
+            api.expert_mm(h, api.DnMat(x), api.DnMat(w), api.DnMat(out))
+        else:
+            api.expert_mm_grad_weight(h, api.DnMat(x), api.DnMat(dz), api.DnMat(out))
+        return api.device_error(h)
+
+    monkeypatch.setenv("ASP_TEST_DROP_COPY", "1")
+    for polls in ("1", "64", "1000"):
+        monkeypatch.setenv("ASP_WAIT_POLLS", polls)
+        assert call(api.Handle()) == 1
+    monkeypatch.delenv("ASP_TEST_DROP_COPY")
+    monkeypatch.delenv("ASP_WAIT_POLLS")
+    out.fill_(float("nan"))
+    assert call(api.Handle()) == 0
+    a, b = (x, w.t()) if kind == "mm" else (dz.t(), x)
+    close(out, a.double() @ b.double(), 2 * U * a.shape[1] * (a.double().abs() @ b.double().abs()))
+
+
 # ---- the epilogue's gradient ---------------------------------------------------------------------
 
 ACT_SHAPES = [([1], 1, 0, 0), ([0, 5, 0], 64, 0, 0), ([127, 2, 128, 300, 0, 1], 264, 8, 8), ([1000], 520, 0, 0), ([40, 260], 1003, 5, 1),
