@@ -377,6 +377,7 @@ __device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int 
   for (int c0 = part * kCols; c0 < x.rows; c0 += PARTS * kCols) {
     TO res[kCols];
     if (a.r && in) load_residual<TO>(a, out_row0 + c0, m, x.rows - c0, res);
+    __syncwarp();  // tensor memory is read by the converged warp; past the last column `in` differs between its lanes
     uint32_t acc[kCols];
     tmem_ld16(tmem + (uint32_t)c0, acc);
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -387,7 +388,7 @@ __device__ __forceinline__ void finish_tile(const MmArgs& a, const Tile& x, int 
       if (c0 + kCols <= x.rows) finish_values<TO, ACT, true>(a, out_row0 + c0, m, kCols, bias, res, v);
       else finish_values<TO, ACT, false>(a, out_row0 + c0, m, x.rows - c0, bias, res, v);
     }
-    __syncwarp();  // tensor memory is read by the converged warp
+    __syncwarp();
   }
 }
 

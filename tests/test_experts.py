@@ -553,6 +553,24 @@ def test_a_row_has_the_same_bits_whatever_its_neighbours_hold(h, rows, n, k, op,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 31, 33, 127, 130, 257, 1300])
+@pytest.mark.parametrize("rows", [3, 50, 2400])
+def test_residual_where_the_last_warp_is_part_full(h, rows, n):
+    """Columns that end inside a warp's 32: only some of its lanes have a residual to read before the accumulator is read by all."""
+    k, g = 96, gen(rows + n)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(torch.float16)
+    w = (torch.randn(n, k, device="cuda", generator=g) * k ** -0.5).to(torch.float16)
+    y_flat, y = strided(torch.zeros(rows, n, device="cuda"), 3, 1)
+    r = torch.randn(rows, n, device="cuda", generator=g)
+    before = y_flat.clone()
+    api.expert_mm(h, api.DnMat(x), api.DnMat(w), api.DnMat(y), None, api.OP_T, None, api.ACT_RELU, api.DnMat(r))
+    z, mag = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    want = z.clamp(min=0) + r.double()
+    close(y, want, (k + 2) * 2 * U * mag + 2 * U * (want.abs() + r.double().abs()))
+    assert untouched(y_flat, y, before)
+
+
+@pytest.mark.gpu
 def test_offsets_outside_the_rows(h):
     """Offsets are clamped to the rows; descending ones give an empty segment."""
     off = torch.tensor([-5, 3, 2, 900], dtype=torch.int32, device="cuda")
