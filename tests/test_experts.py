@@ -708,6 +708,30 @@ def test_act_grad(h, case, act, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[1] * 700 + [0] * 50, [0] * 300 + [9] + [0] * 300, [0] * 1024, [0] * 40 + [700] + [0] * 40 + [3]])
+def test_act_grad_of_empty_segments(h, counts):
+    """dBias of every empty segment is zero, wherever it lies, and dZ may take the place of Z."""
+    n, e, rows, off = 24, len(counts), sum(counts), offsets_of(counts)
+    g = gen(len(counts))
+    dy, z = torch.randn(rows, n, device="cuda", generator=g), torch.randn(rows, n, device="cuda", generator=g)
+    db = torch.full((e, n), float("nan"), device="cuda")
+    dz = torch.zeros(rows, n, device="cuda")
+    DY, Z, DB = api.DnMat(dy), api.DnMat(z), api.DnMat(db)
+    buf = buffer(api.expert_act_grad_buffer_size(h, DY, off, api.ACT_GELU, DB))
+    api.expert_act_grad(h, DY, Z, api.DnMat(dz), off, api.ACT_GELU, DB, buf)
+    c = torch.tensor(counts, device="cuda")
+    assert db[c == 0].eq(0).all()
+    seg = torch.repeat_interleave(torch.arange(e, device="cuda"), c)
+    want = dy.double() * slope64(z.double(), api.ACT_GELU)
+    sums, mag = (torch.zeros(e, n, dtype=torch.float64, device="cuda").index_add_(0, seg, t) for t in (want, want.abs()))
+    err = torch.zeros_like(sums).index_add_(0, seg, 16 * U * dy.double().abs())
+    close(db, sums, (c[:, None] + 2) * 2 * U * mag + err)
+    again = torch.full_like(db, float("nan"))
+    api.expert_act_grad(h, DY, Z, Z, off, api.ACT_GELU, api.DnMat(again), buf)
+    assert torch.equal(z, dz) and torch.equal(again, db)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ACTS[1:])
 def test_act_grad_against_differences(h, act):
     """Central differences of the 64-bit activation: step 1e-4, their error (1e-8 / 6) max|act'''| < 1e-8; away from relu's kink."""
