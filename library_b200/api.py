@@ -66,6 +66,11 @@ class AlphaSparseError(RuntimeError):
         super().__init__(f"{where}: ALPHA_SPARSE_STATUS_{STATUS_NAMES.get(status, status)}")
 
 
+class ArgumentError(ValueError, AssertionError):
+    """A tensor that a call cannot take.  Raised, not asserted: the C calls see addresses only, so without these checks (under
+    ``python -O``) host memory or a short buffer would reach a kernel."""
+
+
 _lib = None
 
 
@@ -161,7 +166,8 @@ class Handle:
 
 class DnVec:
     def __init__(self, t: torch.Tensor):
-        assert t.is_cuda and t.is_contiguous()
+        if not (t.is_cuda and t.is_contiguous()):
+            raise ArgumentError("a vector is a contiguous device tensor")
         self.t = t
         self.d = C.c_void_p()
         _check(load().alphasparseCreateDnVec(C.byref(self.d), C.c_int64(t.numel()),
@@ -181,7 +187,8 @@ class DnVecWindow(DnVec):
     """A vector of logical length ``size`` of which only [first, first + t.numel()) exists, in t."""
 
     def __init__(self, t: torch.Tensor, size: int, first: int):
-        assert t.is_cuda and t.is_contiguous()
+        if not (t.is_cuda and t.is_contiguous()):
+            raise ArgumentError("a vector is a contiguous device tensor")
         self.t = t
         self.size, self.first = size, first
         self.d = C.c_void_p()
@@ -196,7 +203,8 @@ class DnMat:
     contiguous tensor); the other stride is the leading dimension."""
 
     def __init__(self, t: torch.Tensor):
-        assert t.is_cuda and t.dim() == 2 and (t.stride(1) == 1 or t.stride(0) == 1)
+        if not (t.is_cuda and t.dim() == 2 and (t.stride(1) == 1 or t.stride(0) == 1)):
+            raise ArgumentError("a matrix is a 2-D device tensor whose rows or columns are contiguous")
         self.t = t
         self.d = C.c_void_p()
         row = t.stride(1) == 1
@@ -219,11 +227,13 @@ class CsrMatrix:
     """alphasparseSpMatDescr_t over three device tensors (kept alive by this object)."""
 
     def __init__(self, rows, cols, row_ptr: torch.Tensor, col_idx: torch.Tensor, val: torch.Tensor):
-        assert row_ptr.is_cuda and col_idx.is_cuda and val.is_cuda
+        if not (row_ptr.is_cuda and col_idx.is_cuda and val.is_cuda):
+            raise ArgumentError("a CSR matrix is made of device tensors")
         self.rows, self.cols, self.nnz = int(rows), int(cols), int(col_idx.numel())
         self.row_ptr, self.col_idx, self.val = row_ptr, col_idx, val
         rt = {torch.int32: INDEX_I32, torch.int64: INDEX_I64}[row_ptr.dtype]
-        assert col_idx.dtype == torch.int32
+        if col_idx.dtype != torch.int32:
+            raise ArgumentError("column indices are int32")
         self.d = C.c_void_p()
         _check(load().alphasparseCreateCsr(
             C.byref(self.d), C.c_int64(rows), C.c_int64(cols), C.c_int64(self.nnz),
@@ -376,7 +386,8 @@ def spmv_csr_noalloc(row_ptr: torch.Tensor, col_idx: torch.Tensor, val: torch.Te
 
 def coo2csr(coo_row: torch.Tensor, rows: int, out_dtype=torch.int32, stream=None) -> torch.Tensor:
     """Row offsets (rows+1) from ascending int32 COO row indices on the device."""
-    assert coo_row.is_cuda and coo_row.dtype == torch.int32
+    if not (coo_row.is_cuda and coo_row.dtype == torch.int32):
+        raise ArgumentError("row indices are an int32 device tensor")
     out = torch.empty(rows + 1, dtype=out_dtype, device=coo_row.device)
     st = torch.cuda.current_stream().cuda_stream if stream is None else stream
     _check(load().alphasparseXcoo2csr(C.c_void_p(st), C.c_void_p(coo_row.data_ptr()), C.c_int64(coo_row.numel()),
@@ -423,14 +434,16 @@ class Routing:
 
     def __init__(self, expert_ids: torch.Tensor, experts: int, offsets: torch.Tensor | None = None,
                  position: torch.Tensor | None = None):
-        assert expert_ids.is_cuda and expert_ids.dim() == 2 and expert_ids.is_contiguous()
+        if not (expert_ids.is_cuda and expert_ids.dim() == 2 and expert_ids.is_contiguous()):
+            raise ArgumentError("expert_ids is a contiguous tokens x topk device tensor")
         self.tokens, self.topk, self.experts = int(expert_ids.shape[0]), int(expert_ids.shape[1]), int(experts)
         self.expert_ids = expert_ids
         dev = expert_ids.device
         self.offsets = torch.empty(self.experts + 1, dtype=torch.int32, device=dev) if offsets is None else offsets
         self.position = torch.empty(expert_ids.shape, dtype=torch.int32, device=dev) if position is None else position
         for t, n in ((self.offsets, self.experts + 1), (self.position, expert_ids.numel())):
-            assert t.device == dev and t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n
+            if not (t.device == dev and t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n):
+                raise ArgumentError(f"a routing array of {n} contiguous int32 on the ids' device is needed")
         self.d = C.c_void_p()
         it = {torch.int32: INDEX_I32, torch.int64: INDEX_I64}[expert_ids.dtype]
         _check(load().alphasparseCreateRouting(C.byref(self.d), C.c_int64(self.tokens), C.c_int64(self.topk),
@@ -460,13 +473,15 @@ def _workspace(buffer: torch.Tensor | None, needed):
     the operands' alignment: a buffer sized for other operands would be written past its end.)"""
     if buffer is None:
         return None
-    assert buffer.is_cuda and buffer.is_contiguous() and buffer.numel() * buffer.element_size() >= needed()
+    if not (buffer.is_cuda and buffer.is_contiguous() and buffer.numel() * buffer.element_size() >= needed()):
+        raise ArgumentError(f"the workspace is a contiguous device tensor of {needed()} bytes or more")
     return buffer.data_ptr()
 
 
 def _gates(routing: Routing, w: torch.Tensor | None):
     """Pointer of a tokens x topk fp32 array (or NULL)."""
-    assert w is None or (w.is_cuda and w.dtype == torch.float32 and w.is_contiguous() and w.numel() == routing.tokens * routing.topk)
+    if not (w is None or (w.is_cuda and w.dtype == torch.float32 and w.is_contiguous() and w.numel() == routing.tokens * routing.topk)):
+        raise ArgumentError("gate weights are a contiguous fp32 device tensor of tokens x topk")
     return _ptr(w)
 
 
@@ -474,7 +489,8 @@ def _segments(offsets: torch.Tensor | None):
     """(segments, device pointer) of int32 row offsets; None is one segment of all rows."""
     if offsets is None:
         return 1, None
-    assert offsets.is_cuda and offsets.dtype == torch.int32 and offsets.is_contiguous()
+    if not (offsets.is_cuda and offsets.dtype == torch.int32 and offsets.is_contiguous()):
+        raise ArgumentError("segment offsets are a contiguous int32 device tensor")
     return offsets.numel() - 1, offsets.data_ptr()
 
 

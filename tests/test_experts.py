@@ -8,6 +8,9 @@ given 16 roundings.  |gelu'| <= 1.13 and |silu'| <= 1.1 carry an error of Z to Y
 """
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -250,6 +253,47 @@ def test_act_grad_refusals():
     assert lib.alphasparseExpertActGrad_bufferSize(FAKE, C.c_int64(3), off, 2, dy, None, C.byref(size)) == 0 and size.value == 0
     assert lib.alphasparseExpertActGrad_bufferSize(FAKE, C.c_int64(3), off, 2, dy, db, C.byref(size)) == 0 and size.value > 0
     assert lib.alphasparseGetDeviceError(None, None) == 8
+
+
+ARGUMENTS = """
+import torch
+from library_b200 import api
+
+class Stand:  # a device tensor's attributes, without a device
+    is_cuda, dtype, device = True, torch.int32, None
+    def __init__(self, n, contiguous=True): self.n, self.c = n, contiguous
+    def is_contiguous(self): return self.c
+    def numel(self): return self.n
+    def element_size(self): return 4
+    def data_ptr(self): return 4096
+
+class Shape: tokens, topk = 4, 2
+
+host = torch.zeros(4, 2, dtype=torch.int32)
+assert_ran = [False]
+assert assert_ran.__setitem__(0, True) is None
+refused = [lambda: api._workspace(Stand(63), lambda: 256), lambda: api._workspace(Stand(64, False), lambda: 256),
+           lambda: api._workspace(host, lambda: 1), lambda: api._segments(host[0]), lambda: api._segments(Stand(4, False)),
+           lambda: api._gates(Shape, host.float()), lambda: api._gates(Shape, Stand(8)), lambda: api.Routing(host, 4), lambda: api.DnMat(host.float()),
+           lambda: api.DnVec(host.float()), lambda: api.CsrMatrix(4, 2, host, host, host), lambda: api.coo2csr(host, 4)]
+for i, call in enumerate(refused):
+    try:
+        call()
+    except api.ArgumentError:
+        continue
+    raise SystemExit(f"call {i} was not refused")
+if api._workspace(Stand(64), lambda: 256) != 4096 or api._workspace(None, None) is not None:
+    raise SystemExit("a workspace that fits was refused")
+print(assert_ran[0])
+"""
+
+
+@pytest.mark.parametrize("flag", ["-O", "-B"])
+def test_tensors_are_refused_with_and_without_assertions(flag):
+    """The bindings' checks of tensors (host memory, short workspaces, wrong types) hold under python -O."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, flag, "-c", ARGUMENTS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == str(flag != "-O"), r.stdout + r.stderr[-800:]
 
 
 # ---- the sort ---------------------------------------------------------------------------------
