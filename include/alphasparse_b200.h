@@ -552,7 +552,10 @@ alphasparseStatus_t alphasparseRoutingCombineGrad(alphasparseHandle_t handle,
  * accumulation on the tensor cores.  K = 0 is an empty sum.
  * The gradient with respect to X is this call on dZ with the other opW (no bias, no activation).
  * externalBuffer: alphasparseExpertMM_bufferSize bytes (0 for the usual operands: 16-byte aligned
- * X and W with leading dimensions that are multiples of 8; others are copied into it first). */
+ * X and W with leading dimensions that are multiples of 8; others are copied into it first).  The
+ * size holds for these descriptors with these addresses: ask again whenever an operand's values or
+ * leading dimension change (a view that starts off 16 bytes needs more than an aligned one of the
+ * same shape).  The call cannot see how long the buffer is; a shorter one is written past its end. */
 alphasparseStatus_t alphasparseExpertMM(alphasparseHandle_t handle, alphasparseOperation_t opW,
                                         int64_t segments, const int32_t* segOffsets,
                                         alphasparseDnMatDescr_t matX, alphasparseDnMatDescr_t matW,
@@ -568,7 +571,8 @@ alphasparseStatus_t alphasparseExpertMM_bufferSize(alphasparseHandle_t handle,
 /* Gradient with respect to the weights, in the layout of matW (opW as in the forward call):
  *   TRANSPOSE: dW_e = dZ_e^T * X_e (N x K)      NON_TRANSPOSE: dW_e = X_e^T * dZ_e (K x N)
  * over the rows of segment e; an empty segment's block is zero.  X, dZ: R_16BF or R_16F, the same;
- * dW: that type or R_32F.  externalBuffer as in alphasparseExpertMM. */
+ * dW: that type or R_32F.  externalBuffer as in alphasparseExpertMM, for X and dZ: ask again whenever
+ * their addresses change. */
 alphasparseStatus_t alphasparseExpertMM_gradW(alphasparseHandle_t handle, alphasparseOperation_t opW,
                                               int64_t segments, const int32_t* segOffsets,
                                               alphasparseDnMatDescr_t matX,

@@ -255,6 +255,33 @@ def test_act_grad_refusals():
     assert lib.alphasparseGetDeviceError(None, None) == 8
 
 
+def test_workspace_sizes_follow_the_operands_addresses():
+    """The same descriptor, asked again after its values moved off 16 bytes, needs room for a copy: rows x cols rounded up to 8, and 256
+    bytes to align."""
+    lib = api.load()
+    x, w, y, dz, dw = dn(10, 24), dn(3 * 40, 24), dn(10, 40), dn(10, 40), dn(3 * 40, 24)
+    off, size = C.c_void_p(0x1000), C.c_size_t()
+
+    def mm():
+        assert lib.alphasparseExpertMM_bufferSize(FAKE, api.OP_T, C.c_int64(3), off, x, w, y, C.byref(size)) == 0
+        return size.value
+
+    def grad():
+        assert lib.alphasparseExpertMM_gradW_bufferSize(FAKE, api.OP_T, C.c_int64(3), off, x, dz, dw, C.byref(size)) == 0
+        return size.value
+
+    assert mm() == 0 and grad() == 0
+    assert lib.alphasparseDnMatSetValues(x, C.c_void_p(0x1002)) == 0
+    assert mm() >= 10 * 24 * 2 and grad() >= 10 * 24 * 2
+    alone = mm()
+    assert lib.alphasparseDnMatSetValues(w, C.c_void_p(0x1008)) == 0
+    assert mm() >= alone + 3 * 40 * 24 * 2
+    assert lib.alphasparseExpertMM(FAKE, api.OP_T, C.c_int64(3), off, x, w, None, 0, None, None, y, None) == 7
+    for d in (x, w):
+        assert lib.alphasparseDnMatSetValues(d, C.c_void_p(0x1000)) == 0
+    assert mm() == 0 and grad() == 0
+
+
 ARGUMENTS = """
 import torch
 from library_b200 import api
