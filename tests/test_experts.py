@@ -1060,3 +1060,51 @@ def test_offsets_past_32_bits(h):
     z = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
     api.expert_act_grad(h, api.DnMat(x), api.DnMat(z), api.DnMat(x), None, api.ACT_SILU)
     assert torch.equal(x[-1], (out[0].float() * 0.5).to(torch.bfloat16))
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def python(code):
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr[-800:]
+
+
+def test_the_stream_is_asked_of_torch_where_the_short_way_is_missing():
+    python("""
+import torch
+for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+class Stream: cuda_stream = 77
+torch.cuda.current_stream = lambda: Stream
+from library_b200 import api
+assert api._stream_number() == 77
+""")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("short", [True, False])
+def test_a_handle_follows_torchs_stream(short):
+    """A program whose first call is the library's: torch's own state of the device is set up, and the handle takes the
+    current stream, with the short way of asking for it and without."""
+    python(f"""
+import ctypes as C
+import torch
+from library_b200 import api
+h = api.Handle()
+assert torch.cuda.is_initialized() and (api._raw_stream is not None or not {short})
+if not {short}:
+    api._raw_stream = None
+def stream():
+    p = C.c_void_p()
+    assert api.load().alphasparseGetStream(h.h, C.byref(p)) == 0
+    return p.value or 0
+assert stream() == torch.cuda.current_stream().cuda_stream
+s = torch.cuda.Stream()
+with torch.cuda.stream(s):
+    h.use_torch_stream()
+assert stream() == s.cuda_stream != 0
+h.use_torch_stream()
+assert stream() == torch.cuda.current_stream().cuda_stream
+""")
