@@ -205,7 +205,8 @@ constexpr int kEpiParts = 2;                   // epilogue warps per quarter of 
 constexpr int kEpiWarp0 = 4, kEpiWarps = 4 * kEpiParts;
 constexpr int kMmThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;                 // two accumulators of 256 columns
-// Polls of a bounded wait: seconds, and more than a tile of `chunks` stages can take.
+// Polls of a bounded wait: seconds, and more than a tile of `chunks` stages can take.  Below 2^31, so that twice the limit and the
+// peers' margin stay a number of 32 bits.
 inline uint32_t wait_limit(alphasparseHandle_t h, int64_t chunks) {
   const HandleImpl* i = impl(h);
   if (i->expert_wait) return i->expert_wait;
@@ -1123,6 +1124,10 @@ struct MmShape {
 // against 85-87; at 2,048 rows 89 against 87).  Beyond, it is the number of tiles that decides: where pair tiles would leave half of
 // the pairs idle and the small tiles still fit the device at once, the small ones run (one 4,096 x 4,096 layer, 32 / 128 / 256 rows:
 // 15 / 18 / 24 us against 26 / 28 / 29; 512 rows 35 against 30; eight 2,048 x 2,048 layers, 256 rows: 23 against 22).
+// How the rows are spread is not known on the host.  Where most go to one expert, its weights are read once per 16 rows, from L2: at
+// 64 experts x 2,048 x 1,408 and the rule's limit of 1,024 rows 60 us against 69 when they are even, 66 against 70 with half of them at
+// one expert, 77 against 69 with 961; at 512 rows 64 against 68 with 449 at one.  It loses more with more experts: 256 of them, 4,096 rows,
+// 225 against 236 when even, 260 against 243 with half at one, 104 against 29 with all at one.
 int few_rows(alphasparseHandle_t h, const MmShape& s, int64_t filled) {
   const int64_t pairs = (s.rows / kTileJ + filled) * ((s.n + kPairM - 1) / kPairM);
   if (s.rows <= 16 * filled) return 1;
